@@ -29,7 +29,7 @@ CSRC = os.path.join(ROOT, "kaldi_amd", "csrc")
 OUT = os.path.join(ROOT, "build", "regime")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 BASE = ["--offload-arch=gfx950", "-DKAMD_NT=1024", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall",
-        "-Wno-unused-result", "-Wno-pass-failed"]
+        "-Wno-unused-result", "-Wno-pass-failed", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 NO_MLICM = ["-mllvm", "-disable-machine-licm"]          # kaldi_amd/csrc/Makefile: DECODER_FLAGS
 S2M = ["-mllvm", "-amdgpu-spill-sgpr-to-vgpr=0"]
 VARIANTS = {
