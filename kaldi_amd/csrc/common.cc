@@ -81,7 +81,7 @@ struct Bounce {
 // (hipPointerGetAttributes) -- but the runtime's view goes stale: a range that was registered, or that the runtime pinned for a
 // pageable copy and kept in its pin cache, and was then given back to the allocator still reads "hipMemoryTypeHost" when
 // the same addresses come back as another, pageable, buffer, and a copy started on that answer faults the GPU on the first page
-// that is no longer mapped for it (tools/repro/pinned_neighbour.cc scenario 7: "Memory access fault by GPU node-2 ... on
+// that is no longer mapped for it (seen as "Memory access fault by GPU node-2 ... on
 // address <the mapping>", the abort of rounds 4 / 5 word for word).  A caller's own page-locked memory is therefore treated as
 // pageable -- one more memcpy, never a fault.
 std::mutex g_pin_mu;
