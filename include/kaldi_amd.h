@@ -252,6 +252,48 @@ int kamd_component_output_rows(const kamd_component *c, int in_rows);
 int kamd_component_propagate(kamd_component *c, const float *d_in, int in_rows, int ld_in, float *d_out, int ld_out,
                              void *stream);
 
+/* ---------------------------------------------------------- 8-bit layers -- */
+/* Layers whose products run on 8-bit integers: rows normalised and / or coded with one scale per row, weights with one scale
+ * per output channel, sums in 32-bit integers.  All device pointers; asynchronous on `stream`, no workspace, no state between
+ * calls (any number of calls may run at once, and be captured into graphs).  Leading dimensions count elements.  Pointers and
+ * stream belong to the current device.  Element types: */
+enum { KAMD_F32 = 0, KAMD_BF16 = 1, KAMD_F16 = 2, KAMD_I8 = 3 };
+/* NormalizeComponent (nnet3/nnet-normalize-component.cc; NormalizePerRow, cudamatrix/cu-math.cc) with the residual and the
+ * gain of a pre-norm layer, row by row:
+ *   h = x (+ residual),   sum = h,   out = h / sqrt(mean(h^2) + eps) * gain
+ * d_residual, d_gain (float [dim]; NULL = ones; constant target_rms = --target-rms) and d_sum may be NULL.  NormalizeComponent's
+ * floor is eps = 2^-66.  h is the 32-bit sum, also where d_sum rounds it to 16 bits.  out_type is `type`, or KAMD_I8: then out
+ * holds codes in [-127, 127] and d_out_scale[row] their scale: out ~ code * scale, off by at most scale / 2; a row of zeros has
+ * scale 0, one that holds an infinity or a NaN has scale NaN (and codes 0).  d_sum may be d_x or d_residual, and d_out (of the
+ * input's type) any of the three, at the same leading dimension; other overlaps are not allowed. */
+int kamd_rms_norm_device(const void *d_x, int64_t ld_x, const void *d_residual, int64_t ld_residual, int type,
+                         const float *d_gain, float eps, int64_t rows, int dim, void *d_sum, int64_t ld_sum,
+                         void *d_out, int64_t ld_out, int out_type, float *d_out_scale, void *stream);
+/* The 8-bit form of a layer's input: output row j is Append_i x[j + offsets[i] - min(offsets)] (offsets on the host, as in
+ * kamd_layer_desc; {0} for plain rows) as codes and a scale, in_rows - (max - min) rows of n_offsets * dim codes. */
+int kamd_quantize_rows_device(const void *d_x, int64_t ld_x, int type, int64_t in_rows, int dim,
+                              const int32_t *offsets, int n_offsets, int8_t *d_q, int64_t ld_q, float *d_scale,
+                              void *stream);
+/* kamd_component (one fused affine layer) in 8 bits: out = map(sum_k q[row][k] w[n][k] * scale[row] * w_scale[n] + bias[n]),
+ * map = the layer's ReLU, then its BatchNorm and post maps. */
+typedef struct kamd_component_i8 kamd_component_i8;
+/* From a layer description (host float weights): the weights are coded per output channel here.  No multi_input, ivector,
+ * log-softmax; the bypass is ignored as in kamd_component. */
+kamd_component_i8 *kamd_component_i8_create(const kamd_layer_desc *layer);
+/* From weights that are coded already, d_w [out_dim x in_dim] and d_w_scale [out_dim] on the device (copied).  d_bias, d_mul
+ * and d_add [out_dim] may be NULL: out = mul * relu(... + bias) + add. */
+kamd_component_i8 *kamd_component_i8_create_quantized(const int8_t *d_w, int64_t ld_w, const float *d_w_scale, int in_dim,
+                                                      int out_dim, const float *d_bias, int relu, const float *d_mul,
+                                                      const float *d_add, void *stream);
+void kamd_component_i8_destroy(kamd_component_i8 *c);
+int kamd_component_i8_input_dim(const kamd_component_i8 *c);   /* codes per row: n_offsets * in_dim of the layer */
+int kamd_component_i8_output_dim(const kamd_component_i8 *c);
+/* d_q: `rows` rows of codes, 16-byte aligned, ld_q a multiple of 16 (what lies between the row's end and the next multiple of
+ * 16 bytes is read and has no effect); d_scale [rows]; out_type KAMD_F32, KAMD_BF16 or KAMD_F16.  A row's result does not
+ * depend on the other rows of the call. */
+int kamd_component_i8_propagate(const kamd_component_i8 *c, const int8_t *d_q, int64_t ld_q, const float *d_scale,
+                                int64_t rows, void *d_out, int64_t ld_out, int out_type, void *stream);
+
 /* ----------------------------------------------------------------- model -- */
 /* final.mdl -> what the decode path consumes.  Replaces, for this path, what the binary does
  * before it decodes (nnet3bin/nnet3-latgen-faster.cc:91-104): ReadKaldiObject of the

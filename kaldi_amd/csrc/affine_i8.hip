@@ -1,0 +1,389 @@
+// affine_i8.hip -- the affine product in 8-bit integers (kamd_component_i8_*):
+//
+//   out[m][n] = map(sum_k q[m][k] w[n][k] * scale[m] * w_scale[n] + bias[n]),   map(z) = mul[n] * relu(z) + add[n]
+//
+// The sum is exact: products of 8-bit codes in 32-bit integers (at most 131071 of them), by v_mfma_i32_16x16x64_i8.  It is
+// turned into a 32-bit float once and rounded to the output's type once.
+//
+// The weights are laid out once, when the handle is made, in the order in which the matrix units take them: blocks of 16
+// channels x 64 codes, 1 KB each, lane l of a wave holding channel l % 16, codes 16 (l / 16) .. +15, one 16-byte load per lane.
+// A block is contiguous in memory, contiguous in LDS, and read from LDS without a bank conflict.  Channels are padded to
+// kPadN and codes to kPadK with zeros, so that no kernel has to guard a weight, and so that whatever the activations' row holds
+// beyond its last code meets a zero.
+//
+// The weights are operand A (rows = channels) and the activations operand B (columns = rows of the call): a lane then holds
+// four consecutive channels of ONE row, i.e. one row scale and a contiguous piece of the output.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "common.h"
+
+namespace kamd {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+constexpr int kPadN = 256, kPadK = 128;
+constexpr int64_t kMaxIn = 131071;        // 128 * 128 * 131071 < 2^31
+constexpr int64_t kMaxLd = 1 << 23;       // a tile's rows stay within 32-bit offsets of its first
+
+struct AffineI8 {
+  int device = 0, in_dim = 0, out_dim = 0, kp = 0, np = 0, relu = 0, mapped = 0;
+  unsigned char *w = NULL;                // [np / 16][kp / 64][64 lanes][16]
+  float *col = NULL;                      // [4][np]: w_scale, bias, mul, add
+};
+
+struct AffineArgs {
+  const unsigned char *w;
+  const int8_t *q;
+  const float *scale;
+  const float *col;
+  void *out;
+  int64_t ld_q, ld_out;
+  int rows, n, np;
+  int kb;                                 // 64-code blocks per channel = kp / 64
+  int last_chunk;                         // byte offset of a row's last 16-byte chunk that may be read
+  int relu, mapped;
+  int tiles_m, tiles_n;
+};
+
+template <typename V, typename T>
+__device__ inline void StoreAny(T *p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
+
+// four consecutive channels n .. n + 3 of one row
+template <typename TO>
+__device__ inline void FinishFour(const AffineArgs &p, i32x4 acc, float scale, int m, int n) {
+  typedef TO OV __attribute__((ext_vector_type(4)));
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  const f32x4 ws = *reinterpret_cast<const f32x4 *>(p.col + n), b = *reinterpret_cast<const f32x4 *>(p.col + p.np + n);
+  float z[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    z[j] = static_cast<float>(acc[j]) * ws[j] * scale + b[j];
+    if (p.relu) z[j] = z[j] < 0.0f ? 0.0f : z[j];                // (a NaN stays one)
+  }
+  if (p.mapped) {
+    const f32x4 mul = *reinterpret_cast<const f32x4 *>(p.col + 2 * p.np + n), add = *reinterpret_cast<const f32x4 *>(p.col + 3 * p.np + n);
+#pragma unroll
+    for (int j = 0; j < 4; j++) z[j] = z[j] * mul[j] + add[j];
+  }
+  TO *o = static_cast<TO *>(p.out) + m * p.ld_out + n;
+  OV v;
+#pragma unroll
+  for (int j = 0; j < 4; j++) v[j] = static_cast<TO>(z[j]);
+  if (n + 4 <= p.n) StoreAny(o, v);
+  else
+    for (int j = 0; j < 4; j++)
+      if (n + j < p.n) o[j] = v[j];
+}
+
+// Few rows: the weights are read once, straight into registers; nothing is shared, so nothing is staged.  One workgroup per
+// 16 channels, its 8 waves take every 8th block of 64 codes and join their sums in LDS.
+template <int MT, typename TO>
+__global__ __launch_bounds__(512) void FewRowsKernel(AffineArgs p) {
+  constexpr int NW = 8, U = MT <= 2 ? 4 : 2;
+  __shared__ i32x4 part[NW][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned char *w = p.w + static_cast<size_t>(blockIdx.x) * p.kb * 1024 + lane * 16;
+  const int8_t *x[MT];
+#pragma unroll
+  for (int i = 0; i < MT; i++) x[i] = p.q + static_cast<int64_t>(min(i * 16 + (lane & 15), p.rows - 1)) * p.ld_q;
+  const int chunk = (lane >> 4) * 16;
+  i32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; i++) acc[i] = i32x4{0, 0, 0, 0};
+  for (int k0 = wave; k0 < p.kb; k0 += NW * U) {
+    i32x4 a[U], b[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (k0 + u * NW < p.kb) {
+        a[u] = *reinterpret_cast<const i32x4 *>(w + static_cast<size_t>(k0 + u * NW) * 1024);
+        const int at = min((k0 + u * NW) * 64 + chunk, p.last_chunk);
+#pragma unroll
+        for (int i = 0; i < MT; i++) b[u][i] = *reinterpret_cast<const i32x4 *>(x[i] + at);
+      }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (k0 + u * NW < p.kb)
+#pragma unroll
+        for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][i], acc[i], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; i++) part[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave >= MT) return;
+  i32x4 s = part[0][wave][lane];
+#pragma unroll
+  for (int v = 1; v < NW; v++) s += part[v][wave][lane];
+  const int m = wave * 16 + (lane & 15), n = blockIdx.x * 16 + (lane >> 4) * 4;
+  if (m < p.rows && n < p.n) FinishFour<TO>(p, s, p.scale[m], m, n);
+}
+
+// Workgroups are handed to the 8 XCDs in turn.  Each XCD takes one contiguous stretch of the tiles, and the stretch runs
+// through bands of 8 row tiles, so that the tiles that are worked on at once share their operands in the XCD's L2.
+__device__ inline void TileOf(int b, int tiles_m, int tiles_n, int *tm, int *tn) {
+  const int all = tiles_m * tiles_n, xcd = b & 7, each = all >> 3, more = all & 7;
+  const int i = xcd * each + min(xcd, more) + (b >> 3);
+  constexpr int kBand = 8;
+  const int band = i / (kBand * tiles_n), first = band * kBand, high = min(kBand, tiles_m - first), in = i - first * tiles_n;
+  *tm = first + in % high;
+  *tn = in / high;
+}
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+// BM rows x BN channels per workgroup of WM x WN waves; stages of 128 codes, NST of them in LDS.
+template <int BM, int BN, int WM, int WN, int NST, typename TO>
+__global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
+  constexpr int NW = WM * WN, TI = BM / WM / 16, TJ = BN / WN / 16;
+  constexpr int X_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = X_BYTES + W_BYTES;
+  constexpr int X_PW = BM / 8 / NW, W_PW = BN / 8 / NW, LOADS = X_PW + W_PW;       // 1 KB loads of a wave per stage
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BN <= kPadN, "tile");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[NST * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  TileOf(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * BN, rows = min(BM, p.rows - m0);
+  const unsigned lds = static_cast<unsigned>(reinterpret_cast<size_t>((lds_byte *)smem));
+
+  // Buffer descriptors: base, extent, raw 32-bit data.  Every offset below stays inside by itself (rows clamped to the last
+  // one, chunks to last_chunk).
+  const size_t xb = reinterpret_cast<size_t>(p.q + static_cast<int64_t>(m0) * p.ld_q), wb = reinterpret_cast<size_t>(p.w + static_cast<size_t>(n0) * p.kb * 64);
+  i32x4 xr = {static_cast<int>(xb), static_cast<int>((xb >> 32) & 0xffff), static_cast<int>((rows - 1) * p.ld_q + p.last_chunk + 16), 0x00027000};
+  i32x4 wr = {static_cast<int>(wb), static_cast<int>((wb >> 32) & 0xffff), BN * p.kb * 64, 0x00027000};
+#pragma unroll
+  for (int i = 0; i < 4; i++) { xr[i] = __builtin_amdgcn_readfirstlane(xr[i]); wr[i] = __builtin_amdgcn_readfirstlane(wr[i]); }
+
+  // Activations: a load covers 8 rows x 128 codes.  Chunk c (16 codes) of row r goes to slot c ^ ((r >> 1) & 7) of the row, so
+  // that the 16 lanes that read one chunk of 16 rows touch all 64 banks once.
+  int x_row[X_PW], x_chunk[X_PW];
+#pragma unroll
+  for (int i = 0; i < X_PW; i++) {
+    const int r = (wave + NW * i) * 8 + (lane >> 3);
+    x_row[i] = min(r, rows - 1) * static_cast<int>(p.ld_q);
+    x_chunk[i] = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+  }
+  auto load = [&](unsigned to, i32x4 rsrc, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+  };
+  auto issue = [&](int kt, int stage) {
+    const unsigned at = lds + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < X_PW; i++) load(at + (wave + NW * i) * 1024, xr, x_row[i] + min(kt * 128 + x_chunk[i], p.last_chunk), 0);
+#pragma unroll
+    for (int i = 0; i < W_PW; i++) {
+      const int j = wave + NW * i;                               // block j / 2 of 16 channels, half j % 2 of the 128 codes
+      load(at + X_BYTES + j * 1024, wr, lane * 16, ((j >> 1) * p.kb + kt * 2 + (j & 1)) * 1024);
+    }
+  };
+
+  i32x4 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; i++)
+#pragma unroll
+    for (int j = 0; j < TJ; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+  const int steps = p.kb >> 1;
+#pragma unroll
+  for (int s = 0; s < NST - 1; s++)
+    if (s < steps) issue(s, s);
+  const int xoff = (lane & 15) * 128, xslot = (lane >> 4) ^ ((lane >> 1) & 7);
+  int stage = 0;
+  for (int kt = 0; kt < steps; kt++) {
+    if (NST > 2 && kt + NST - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                                // this stage is there, and the one before has been read by all
+    asm volatile("" ::: "memory");
+    if (kt + NST - 1 < steps) issue(kt + NST - 1, stage == 0 ? NST - 1 : stage - 1);
+    const unsigned char *xs = smem + stage * STAGE + wm * (BM / WM) * 128 + xoff;
+    const unsigned char *ws = smem + stage * STAGE + X_BYTES + wn * (BN / WN / 16) * 2048 + lane * 16;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      i32x4 a[TJ], b[TI];
+#pragma unroll
+      for (int j = 0; j < TJ; j++) a[j] = *reinterpret_cast<const i32x4 *>(ws + (j * 2 + h) * 1024);
+#pragma unroll
+      for (int i = 0; i < TI; i++) b[i] = *reinterpret_cast<const i32x4 *>(xs + i * 2048 + ((xslot ^ (h * 4)) * 16));
+#pragma unroll
+      for (int i = 0; i < TI; i++)
+#pragma unroll
+        for (int j = 0; j < TJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], b[i], acc[i][j], 0, 0, 0);
+    }
+    stage = stage + 1 == NST ? 0 : stage + 1;
+  }
+#pragma unroll
+  for (int i = 0; i < TI; i++) {
+    const int m = m0 + wm * (BM / WM) + i * 16 + (lane & 15);
+    if (m >= p.rows) continue;
+    const float scale = p.scale[m];
+#pragma unroll
+    for (int j = 0; j < TJ; j++) {
+      const int n = n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4;
+      if (n < p.n) FinishFour<TO>(p, acc[i][j], scale, m, n);
+    }
+  }
+}
+
+// [n x k] codes -> the layout above; one thread per 16 codes
+__global__ __launch_bounds__(256) void PackKernel(const int8_t *w, int64_t ld, int n, int k, int kb, unsigned char *to, int64_t chunks) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= chunks) return;
+  const int lane = static_cast<int>(i & 63);
+  const int64_t block = i >> 6;
+  const int row = static_cast<int>(block / kb) * 16 + (lane & 15), at = static_cast<int>(block % kb) * 64 + (lane >> 4) * 16;
+  int8_t v[16];
+#pragma unroll
+  for (int j = 0; j < 16; j++) v[j] = row < n && at + j < k ? w[row * ld + at + j] : 0;
+  __builtin_memcpy(to + i * 16, v, 16);
+}
+
+// the four vectors of the output channels, padded to np; NULL = the neutral value
+__global__ __launch_bounds__(256) void ColumnsKernel(const float *w_scale, const float *bias, const float *mul, const float *add, int n, int np, float *to) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= np) return;
+  const bool in = i < n;
+  to[i] = in ? w_scale[i] : 0.0f;
+  to[np + i] = in && bias ? bias[i] : 0.0f;
+  to[2 * np + i] = in && mul ? mul[i] : 1.0f;
+  to[3 * np + i] = in && add ? add[i] : 0.0f;
+}
+
+template <typename TO>
+int Propagate(const AffineArgs &a, hipStream_t st) {
+  AffineArgs p = a;
+  if (p.rows <= 64) {
+    const dim3 grid(CeilDiv(p.n, 16));
+    if (p.rows <= 16) hipLaunchKernelGGL((FewRowsKernel<1, TO>), grid, dim3(512), 0, st, p);
+    else if (p.rows <= 32) hipLaunchKernelGGL((FewRowsKernel<2, TO>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((FewRowsKernel<4, TO>), grid, dim3(512), 0, st, p);
+  } else {
+    p.tiles_m = CeilDiv(p.rows, 128); p.tiles_n = CeilDiv(p.n, 128);
+    hipLaunchKernelGGL((TileKernel<128, 128, 2, 2, 2, TO>), dim3(p.tiles_m * p.tiles_n), dim3(256), 0, st, p);
+  }
+  KAMD_HIP(hipGetLastError());
+  return KAMD_OK;
+}
+
+void Free(AffineI8 *c) {
+  if (!c) return;
+  if (c->w) (void)hipFree(c->w);
+  if (c->col) (void)hipFree(c->col);
+  delete c;
+}
+
+int CheckSizes(const char *who, int64_t in_dim, int64_t out_dim) {
+  if (in_dim < 1 || out_dim < 1) return SetError(KAMD_ERR_ARG, "%s: bad sizes (%lld -> %lld)", who, static_cast<long long>(in_dim), static_cast<long long>(out_dim));
+  if (in_dim > kMaxIn) return SetError(KAMD_ERR_ARG, "%s: %lld inputs: a 32-bit sum of 8-bit products holds at most %lld", who, static_cast<long long>(in_dim), static_cast<long long>(kMaxIn));
+  if (out_dim > INT32_MAX - kPadN) return SetError(KAMD_ERR_ARG, "%s: too many outputs (%lld)", who, static_cast<long long>(out_dim));
+  return KAMD_OK;
+}
+
+}  // namespace
+}  // namespace kamd
+using kamd::AffineI8;
+using kamd::SetError;
+
+extern "C" {
+
+kamd_component_i8 *kamd_component_i8_create_quantized(const int8_t *d_w, int64_t ld_w, const float *d_w_scale, int in_dim, int out_dim,
+                                                      const float *d_bias, int relu, const float *d_mul, const float *d_add, void *stream) {
+  if (kamd::CheckSizes("kamd_component_i8_create_quantized", in_dim, out_dim) != KAMD_OK) return NULL;
+  if (!d_w || !d_w_scale || ld_w < in_dim) { SetError(KAMD_ERR_ARG, "kamd_component_i8_create_quantized: null argument or leading dimension smaller than the matrix"); return NULL; }
+  if (!kamd::RequireDevice()) return NULL;
+  AffineI8 *c = new (std::nothrow) AffineI8();
+  if (!c) { SetError(KAMD_ERR_HIP, "kamd_component_i8_create_quantized: out of memory"); return NULL; }
+  c->in_dim = in_dim; c->out_dim = out_dim; c->kp = kamd::RoundUp(in_dim, kamd::kPadK); c->np = kamd::RoundUp(out_dim, kamd::kPadN);
+  c->relu = relu != 0; c->mapped = d_mul || d_add;
+  const size_t bytes = static_cast<size_t>(c->np) * c->kp;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = hipGetDevice(&c->device);
+  if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&c->w), bytes);
+  if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&c->col), sizeof(float) * 4 * c->np);
+  if (e == hipSuccess) {
+    hipLaunchKernelGGL(kamd::PackKernel, dim3(kamd::CeilDiv(static_cast<int64_t>(bytes / 16), 256)), dim3(256), 0, st, d_w, ld_w, out_dim, in_dim, c->kp / 64,
+                       c->w, static_cast<int64_t>(bytes / 16));
+    hipLaunchKernelGGL(kamd::ColumnsKernel, dim3(kamd::CeilDiv(c->np, 256)), dim3(256), 0, st, d_w_scale, d_bias, d_mul, d_add, out_dim, c->np, c->col);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess) e = hipStreamSynchronize(st);             // the caller's arrays may go, and any stream may use the handle
+  if (e != hipSuccess) {
+    SetError(KAMD_ERR_HIP, "kamd_component_i8_create_quantized: %s", hipGetErrorString(e));
+    kamd::Free(c);
+    return NULL;
+  }
+  return reinterpret_cast<kamd_component_i8 *>(c);
+}
+
+kamd_component_i8 *kamd_component_i8_create(const kamd_layer_desc *layer) {
+  if (!layer || layer->ivector_dim != 0 || layer->multi_input || layer->log_softmax || layer->n_offsets < 1 || layer->n_offsets > KAMD_MAX_OFFSETS || !layer->W) {
+    SetError(KAMD_ERR_ARG, "kamd_component_i8_create: a plain fused layer is expected (weights; no ivector, multi_input or log-softmax)");
+    return NULL;
+  }
+  const int64_t k = static_cast<int64_t>(layer->in_dim) * layer->n_offsets;
+  const int n = layer->out_dim;
+  if (kamd::CheckSizes("kamd_component_i8_create", layer->in_dim < 1 ? 0 : k, n) != KAMD_OK) return NULL;
+  const size_t values = static_cast<size_t>(n) * k;
+  for (size_t i = 0; i < values; i++)
+    if (!std::isfinite(layer->W[i])) { SetError(KAMD_ERR_ARG, "kamd_component_i8_create: weight %zu is not finite", i); return NULL; }
+  if (!kamd::RequireDevice()) return NULL;
+  // weights, their codes and scales, and the channel vectors: one allocation, released below
+  const size_t f_w = values, f_col = static_cast<size_t>(n) * 4, bytes = (f_w + f_col) * 4 + values;
+  float *d = NULL;
+  hipError_t e = hipMalloc(reinterpret_cast<void **>(&d), bytes);
+  if (e != hipSuccess) { SetError(KAMD_ERR_HIP, "kamd_component_i8_create: %s", hipGetErrorString(e)); return NULL; }
+  float *d_scale = d + f_w, *d_bias = d_scale + n, *d_mul = d_bias + n, *d_add = d_mul + n;
+  int8_t *d_q = reinterpret_cast<int8_t *>(d_add + n);
+  // BatchNorm and post maps: (bn_scale * z + bn_offset + post_offset) * post_scale
+  const bool mapped = layer->bn_scale || layer->bn_offset || layer->post_offset || layer->post_scale != 1.0f;
+  kamd_component_i8 *c = NULL;
+  try {
+    std::vector<float> mul(n), add(n);
+    for (int i = 0; i < n; i++) {
+      mul[i] = (layer->bn_scale ? layer->bn_scale[i] : 1.0f) * layer->post_scale;
+      add[i] = ((layer->bn_offset ? layer->bn_offset[i] : 0.0f) + (layer->post_offset ? layer->post_offset[i] : 0.0f)) * layer->post_scale;
+    }
+    e = hipMemcpy(d, layer->W, values * 4, hipMemcpyHostToDevice);
+    if (e == hipSuccess && layer->bias) e = hipMemcpy(d_bias, layer->bias, sizeof(float) * n, hipMemcpyHostToDevice);
+    if (e == hipSuccess && mapped) e = hipMemcpy(d_mul, mul.data(), sizeof(float) * n, hipMemcpyHostToDevice);
+    if (e == hipSuccess && mapped) e = hipMemcpy(d_add, add.data(), sizeof(float) * n, hipMemcpyHostToDevice);
+    const int32_t zero = 0;
+    if (e != hipSuccess) SetError(KAMD_ERR_HIP, "kamd_component_i8_create: %s", hipGetErrorString(e));
+    else if (kamd_quantize_rows_device(d, k, KAMD_F32, n, static_cast<int>(k), &zero, 1, d_q, k, d_scale, NULL) == KAMD_OK)
+      c = kamd_component_i8_create_quantized(d_q, k, d_scale, static_cast<int>(k), n, layer->bias ? d_bias : NULL, layer->relu, mapped ? d_mul : NULL,
+                                             mapped ? d_add : NULL, NULL);
+  } catch (const std::exception &) {
+    SetError(KAMD_ERR_HIP, "kamd_component_i8_create: out of memory");
+  }
+  (void)hipFree(d);
+  return c;
+}
+
+void kamd_component_i8_destroy(kamd_component_i8 *h) { kamd::Free(reinterpret_cast<AffineI8 *>(h)); }
+int kamd_component_i8_input_dim(const kamd_component_i8 *h) { return reinterpret_cast<const AffineI8 *>(h)->in_dim; }
+int kamd_component_i8_output_dim(const kamd_component_i8 *h) { return reinterpret_cast<const AffineI8 *>(h)->out_dim; }
+
+int kamd_component_i8_propagate(const kamd_component_i8 *h, const int8_t *d_q, int64_t ld_q, const float *d_scale, int64_t rows, void *d_out,
+                                int64_t ld_out, int out_type, void *stream) {
+  const AffineI8 *c = reinterpret_cast<const AffineI8 *>(h);
+  if (!c || rows < 0 || rows > INT32_MAX - kamd::kPadN) return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: null handle or bad number of rows (%lld)", static_cast<long long>(rows));
+  if (out_type != KAMD_F32 && out_type != KAMD_BF16 && out_type != KAMD_F16) return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: unknown output type %d", out_type);
+  if (ld_q < c->in_dim || ld_out < c->out_dim) return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: leading dimension smaller than the matrix");
+  if (ld_q % 16 != 0 || ld_q > kamd::kMaxLd || reinterpret_cast<uintptr_t>(d_q) % 16 != 0)
+    return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: rows of codes begin on multiples of 16 bytes, at most %lld apart", static_cast<long long>(kamd::kMaxLd));
+  if (rows == 0) return KAMD_OK;
+  if (!d_q || !d_scale || !d_out) return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: null argument");
+  int device = -1;
+  KAMD_HIP(hipGetDevice(&device));
+  if (device != c->device) return SetError(KAMD_ERR_STATE, "kamd_component_i8_propagate: the handle belongs to device %d, the current one is %d", c->device, device);
+  kamd::AffineArgs a = {};
+  a.w = c->w; a.q = d_q; a.scale = d_scale; a.col = c->col; a.out = d_out; a.ld_q = ld_q; a.ld_out = ld_out;
+  a.rows = static_cast<int>(rows); a.n = c->out_dim; a.np = c->np; a.kb = c->kp / 64; a.last_chunk = kamd::RoundUp(c->in_dim, 16) - 16;
+  a.relu = c->relu; a.mapped = c->mapped;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (out_type == KAMD_F32) return kamd::Propagate<float>(a, st);
+  if (out_type == KAMD_BF16) return kamd::Propagate<__bf16>(a, st);
+  return kamd::Propagate<_Float16>(a, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,93 @@
+"""The 8-bit layers' refusals and their C-ABI, without a GPU: every check of arguments comes before the device is touched."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch          # before the library: they share one HIP runtime then
+
+from kaldi_amd import abi
+from kaldi_amd._lib import lib
+from kaldi_amd.nnet import Layer, Model
+
+P = C.c_void_p(1 << 20)         # stands for a device pointer: nothing may read it
+F32, BF16, F16, I8 = 0, 1, 2, 3
+ERR_ARG = -1
+
+
+def norm(x=P, ld_x=8, residual=None, ld_r=0, type=F32, gain=None, eps=1e-6, rows=4, dim=8, sum=None, ld_sum=0, out=P, ld_out=8, out_type=F32, scale=None):
+    return lib().kamd_rms_norm_device(x, ld_x, residual, ld_r, type, gain, eps, rows, dim, sum, ld_sum, out, ld_out, out_type, scale, None)
+
+
+def quantize(x=P, ld_x=8, type=F32, rows=4, dim=8, offsets=(0,), n=None, q=P, ld_q=None, scale=P):
+    off = (C.c_int32 * max(1, len(offsets)))(*offsets)
+    n = len(offsets) if n is None else n
+    return lib().kamd_quantize_rows_device(x, ld_x, type, rows, dim, off, n, q, dim * len(offsets) if ld_q is None else ld_q, scale, None)
+
+
+@pytest.mark.parametrize("bad, says", [
+    (dict(type=3), "input type"), (dict(type=-1), "input type"), (dict(out_type=BF16), "8 bits"), (dict(rows=-1), "sizes"), (dict(dim=0), "sizes"),
+    (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"), (dict(eps=1e-40), "eps"),
+    (dict(ld_x=7), "leading"), (dict(ld_out=7), "leading"), (dict(residual=P, ld_r=7), "leading"), (dict(sum=P, ld_sum=7), "leading"),
+    (dict(x=None), "null"), (dict(out=None), "null"), (dict(out_type=I8), "d_out_scale"),
+])
+def test_rms_norm_refuses(bad, says):
+    assert norm(**bad) == ERR_ARG
+    assert says in lib().kamd_last_error().decode()
+
+
+def test_calls_without_rows_do_nothing():
+    assert norm(rows=0, x=None, out=None) == 0
+    assert quantize(rows=0, x=None) == 0
+    assert quantize(rows=2, offsets=(-1, 0, 1), x=None) == 0        # no row has its context
+    assert quantize(rows=6, offsets=(-3, 3), x=None) == 0
+
+
+@pytest.mark.parametrize("bad, says", [
+    (dict(type=3), "input type"), (dict(rows=-1), "sizes"), (dict(dim=0), "sizes"), (dict(n=0), "sizes"), (dict(n=9), "sizes"),
+    (dict(dim=1 << 30, ld_x=1 << 30, offsets=(0, 1, 2), ld_q=1 << 32), "too long"), (dict(offsets=(-2 ** 31, 2 ** 31 - 1)), "far apart"),
+    (dict(ld_x=7), "leading"), (dict(ld_q=7), "leading"), (dict(offsets=(0, 1), ld_q=15), "leading"), (dict(x=None), "null"), (dict(q=None), "null"), (dict(scale=None), "null"),
+])
+def test_quantize_rows_refuses(bad, says):
+    assert quantize(**bad) == ERR_ARG
+    assert says in lib().kamd_last_error().decode()
+
+
+def test_component_i8_refuses():
+    L = lib()
+
+    def made(ld=8, in_dim=8, out_dim=4, w=P, scale=P):
+        return L.kamd_component_i8_create_quantized(w, ld, scale, in_dim, out_dim, None, 0, None, None, None)
+
+    for kw, says in ((dict(in_dim=0), "sizes"), (dict(out_dim=0), "sizes"), (dict(in_dim=131072, ld=131072), "131071"), (dict(ld=7), "leading"),
+                     (dict(w=None), "null"), (dict(scale=None), "null"), (dict(out_dim=2 ** 31 - 1), "too many")):
+        assert not made(**kw)
+        assert says in L.kamd_last_error().decode(), kw
+    W = np.ones((4, 8), np.float32)
+    for layer, says in ((Layer("a", 8, 4, [0], -1, W, log_softmax=True), "plain"), (Layer("a", 4, 4, [0], -1, W, ivector_dim=4), "plain"),
+                        (Layer("a", 8, 4, [0, 0], -1, W, slice_layers=[0, 1], slice_dims=[4, 4]), "plain")):
+        assert not L.kamd_component_i8_create(Model([layer], 8, 0, 1, 4).descs())
+        assert says in L.kamd_last_error().decode()
+    assert not L.kamd_component_i8_create(None)
+    for v in (np.nan, np.inf):
+        W2 = W.copy()
+        W2[2, 3] = v
+        assert not L.kamd_component_i8_create(Model([Layer("a", 8, 4, [0], -1, W2)], 8, 0, 1, 4).descs())
+        assert "weight 19 is not finite" in L.kamd_last_error().decode()
+    assert L.kamd_component_i8_propagate(None, P, 16, P, 1, P, 16, F32, None) == ERR_ARG
+    L.kamd_component_i8_destroy(None)
+
+
+def test_tensors_off_the_gpu_are_refused():
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    x = torch.zeros(3, 8)
+    for call in (lambda: int8.rms_norm(x), lambda: int8.rms_norm_int8(x), lambda: int8.quantize_rows(x), lambda: int8.quantize_rows(np.zeros((3, 8))),
+                 lambda: int8.AffineInt8(x.to(torch.int8), torch.ones(3))):
+        with pytest.raises(KamdError, match="on the GPU"):
+            call()
+
+
+def test_element_types_match_the_header():
+    from kaldi_amd import int8
+    assert int8._TYPES == {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16} and int8._I8 == I8
+    assert abi.KAMD_MAX_OFFSETS == 8
