@@ -7,7 +7,9 @@
 //
 // The weights are laid out once, when the handle is made, in the order in which the matrix units take them: blocks of 16
 // channels x 64 codes, 1 KB each, lane l of a wave holding channel l % 16, codes 16 (l / 16) .. +15, one 16-byte load per lane.
-// A block is contiguous in memory, contiguous in LDS, and read from LDS without a bank conflict.  Channels are padded to
+// A block is contiguous in memory, contiguous in LDS, and read from LDS without a bank conflict.  The 16 blocks of 256 channels
+// that meet the same 64 codes lie side by side: a tile's stage is one stretch of memory, spread over all channels of the L2
+// (with the blocks of one channel group side by side instead, they lay a power of two apart).  Channels are padded to
 // kPadN and codes to kPadK with zeros, so that no kernel has to guard a weight, and so that whatever the activations' row holds
 // beyond its last code meets a zero.
 //
@@ -16,6 +18,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "common.h"
@@ -30,7 +33,7 @@ constexpr int64_t kMaxLd = 1 << 23;       // a tile's rows stay within 32-bit of
 
 struct AffineI8 {
   int device = 0, in_dim = 0, out_dim = 0, kp = 0, np = 0, relu = 0, mapped = 0;
-  unsigned char *w = NULL;                // [np / 16][kp / 64][64 lanes][16]
+  unsigned char *w = NULL;                // [np / 256][kp / 64][16][64 lanes][16]
   float *col = NULL;                      // [4][np]: w_scale, bias, mul, add
 };
 
@@ -51,16 +54,14 @@ struct AffineArgs {
 template <typename V, typename T>
 __device__ inline void StoreAny(T *p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
-// four consecutive channels n .. n + 3 of one row
-template <typename TO>
-__device__ inline void FinishFour(const AffineArgs &p, i32x4 acc, float scale, int m, int n) {
-  typedef TO OV __attribute__((ext_vector_type(4)));
-  typedef float f32x4 __attribute__((ext_vector_type(4)));
-  const f32x4 ws = *reinterpret_cast<const f32x4 *>(p.col + n), b = *reinterpret_cast<const f32x4 *>(p.col + p.np + n);
-  float z[4];
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// the output of four consecutive channels n .. n + 3 (n < np) of one row, from their sums
+__device__ inline f32x4 Finish(const AffineArgs &p, i32x4 acc, float scale, f32x4 w_scale, f32x4 bias, int n) {
+  f32x4 z;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    z[j] = static_cast<float>(acc[j]) * ws[j] * scale + b[j];
+    z[j] = static_cast<float>(acc[j]) * w_scale[j] * scale + bias[j];
     if (p.relu) z[j] = z[j] < 0.0f ? 0.0f : z[j];                // (a NaN stays one)
   }
   if (p.mapped) {
@@ -68,56 +69,18 @@ __device__ inline void FinishFour(const AffineArgs &p, i32x4 acc, float scale, i
 #pragma unroll
     for (int j = 0; j < 4; j++) z[j] = z[j] * mul[j] + add[j];
   }
-  TO *o = static_cast<TO *>(p.out) + m * p.ld_out + n;
-  OV v;
-#pragma unroll
-  for (int j = 0; j < 4; j++) v[j] = static_cast<TO>(z[j]);
-  if (n + 4 <= p.n) StoreAny(o, v);
-  else
-    for (int j = 0; j < 4; j++)
-      if (n + j < p.n) o[j] = v[j];
+  return z;
 }
 
-// Few rows: the weights are read once, straight into registers; nothing is shared, so nothing is staged.  One workgroup per
-// 16 channels, its 8 waves take every 8th block of 64 codes and join their sums in LDS.
-template <int MT, typename TO>
-__global__ __launch_bounds__(512) void FewRowsKernel(AffineArgs p) {
-  constexpr int NW = 8, U = MT <= 2 ? 4 : 2;
-  __shared__ i32x4 part[NW][MT][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned char *w = p.w + static_cast<size_t>(blockIdx.x) * p.kb * 1024 + lane * 16;
-  const int8_t *x[MT];
+// values n .. n + VE - 1 of a row of the output; those behind its end are dropped
+template <int VE, typename TO, typename V>
+__device__ inline void StoreRow(const AffineArgs &p, int m, int n, V v) {
+  TO *o = static_cast<TO *>(p.out) + m * p.ld_out + n;
+  if (n + VE <= p.n) StoreAny(o, v);
+  else
 #pragma unroll
-  for (int i = 0; i < MT; i++) x[i] = p.q + static_cast<int64_t>(min(i * 16 + (lane & 15), p.rows - 1)) * p.ld_q;
-  const int chunk = (lane >> 4) * 16;
-  i32x4 acc[MT];
-#pragma unroll
-  for (int i = 0; i < MT; i++) acc[i] = i32x4{0, 0, 0, 0};
-  for (int k0 = wave; k0 < p.kb; k0 += NW * U) {
-    i32x4 a[U], b[U][MT];
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      if (k0 + u * NW < p.kb) {
-        a[u] = *reinterpret_cast<const i32x4 *>(w + static_cast<size_t>(k0 + u * NW) * 1024);
-        const int at = min((k0 + u * NW) * 64 + chunk, p.last_chunk);
-#pragma unroll
-        for (int i = 0; i < MT; i++) b[u][i] = *reinterpret_cast<const i32x4 *>(x[i] + at);
-      }
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      if (k0 + u * NW < p.kb)
-#pragma unroll
-        for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][i], acc[i], 0, 0, 0);
-  }
-#pragma unroll
-  for (int i = 0; i < MT; i++) part[wave][i][lane] = acc[i];
-  __syncthreads();
-  if (wave >= MT) return;
-  i32x4 s = part[0][wave][lane];
-#pragma unroll
-  for (int v = 1; v < NW; v++) s += part[v][wave][lane];
-  const int m = wave * 16 + (lane & 15), n = blockIdx.x * 16 + (lane >> 4) * 4;
-  if (m < p.rows && n < p.n) FinishFour<TO>(p, s, p.scale[m], m, n);
+    for (int j = 0; j < VE; j++)
+      if (n + j < p.n) o[j] = v[j];
 }
 
 // Workgroups are handed to the 8 XCDs in turn.  Each XCD takes one contiguous stretch of the tiles, and the stretch runs
@@ -131,9 +94,79 @@ __device__ inline void TileOf(int b, int tiles_m, int tiles_n, int *tm, int *tn)
   *tn = in / high;
 }
 
+// Few rows, or few tiles: what counts is how many loads are under way at once.  A workgroup computes 16 TI rows x 16 TJ channels;
+// each of its 8 waves takes every 8th block of 64 codes of all of them, operands straight into registers, with no barrier until
+// the sums are joined in LDS.
+template <int TI, int TJ, typename TO>
+__global__ __launch_bounds__(512) void SplitKernel(AffineArgs p) {
+  constexpr int NW = 8, U = TI * TJ <= 2 ? 4 : 2;                // U blocks are loaded before the first is multiplied
+  __shared__ i32x4 part[NW][TI * TJ][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  TileOf(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int m0 = tm * TI * 16, n0 = tn * TJ * 16;
+  const unsigned char *w = p.w + (static_cast<size_t>(n0 / kPadN) * p.kb * 16 + n0 % kPadN / 16) * 1024 + lane * 16;
+  const int8_t *x[TI];
+#pragma unroll
+  for (int i = 0; i < TI; i++) x[i] = p.q + static_cast<int64_t>(min(m0 + i * 16 + (lane & 15), p.rows - 1)) * p.ld_q;
+  const int chunk = (lane >> 4) * 16;
+  i32x4 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; i++)
+#pragma unroll
+    for (int j = 0; j < TJ; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+  for (int k0 = wave; k0 < p.kb; k0 += NW * U) {
+    i32x4 a[U][TJ], b[U][TI];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (k0 + u * NW < p.kb) {
+        const int k = k0 + u * NW, at = min(k * 64 + chunk, p.last_chunk);
+#pragma unroll
+        for (int j = 0; j < TJ; j++) a[u][j] = *reinterpret_cast<const i32x4 *>(w + (static_cast<size_t>(k) * 16 + j) * 1024);
+#pragma unroll
+        for (int i = 0; i < TI; i++) b[u][i] = *reinterpret_cast<const i32x4 *>(x[i] + at);
+      }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (k0 + u * NW < p.kb)
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+          for (int j = 0; j < TJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][j], b[u][i], acc[i][j], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < TI; i++)
+#pragma unroll
+    for (int j = 0; j < TJ; j++) part[wave][i * TJ + j][lane] = acc[i][j];
+  __syncthreads();
+  typedef TO OV __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int f0 = 0; f0 < TI * TJ; f0 += NW) {
+    const int f = f0 + wave, m = m0 + f / TJ * 16 + (lane & 15), n = n0 + f % TJ * 16 + (lane >> 4) * 4;
+    if (f >= TI * TJ || m >= p.rows || n >= p.n) continue;
+    i32x4 s = part[0][f][lane];
+#pragma unroll
+    for (int v = 1; v < NW; v++) s += part[v][f][lane];
+    const f32x4 z = Finish(p, s, p.scale[m], *reinterpret_cast<const f32x4 *>(p.col + n), *reinterpret_cast<const f32x4 *>(p.col + p.np + n), n);
+    StoreRow<4, TO>(p, m, n, __builtin_convertvector(z, OV));
+  }
+}
+
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
-// BM rows x BN channels per workgroup of WM x WN waves; stages of 128 codes, NST of them in LDS.
+// s_waitcnt: all but the newest LOADS * `stages` of this wave's loads are there (stages <= MOST), and its LDS reads
+template <int LOADS, int MOST>
+__device__ inline void WaitBut(int stages) {
+  static_assert(LOADS * MOST < 64, "vmcnt has 6 bits");
+  if constexpr (MOST > 0) {
+    if (stages < MOST) return WaitBut<LOADS, MOST - 1>(stages);
+  }
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * MOST) : "memory");
+}
+
+// Many rows: BM rows x BN channels per workgroup of WM x WN waves, operands by DMA into a ring of NST stages of 128 codes in LDS.
+// The product is bound by the power that the matrix units draw: 16384 x 8192 x 8192 runs at 2.6 PFLOP/s with the clock at
+// 2.0 GHz of 2.4, against 3.5 when the operands stay in registers and 4.6 for the matrix instructions alone.
 template <int BM, int BN, int WM, int WN, int NST, typename TO>
 __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   constexpr int NW = WM * WN, TI = BM / WM / 16, TJ = BN / WN / 16;
@@ -150,9 +183,9 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
 
   // Buffer descriptors: base, extent, raw 32-bit data.  Every offset below stays inside by itself (rows clamped to the last
   // one, chunks to last_chunk).
-  const size_t xb = reinterpret_cast<size_t>(p.q + static_cast<int64_t>(m0) * p.ld_q), wb = reinterpret_cast<size_t>(p.w + static_cast<size_t>(n0) * p.kb * 64);
+  const size_t xb = reinterpret_cast<size_t>(p.q + static_cast<int64_t>(m0) * p.ld_q), wb = reinterpret_cast<size_t>(p.w + static_cast<size_t>(n0 / kPadN) * p.kb * (kPadN * 64));
   i32x4 xr = {static_cast<int>(xb), static_cast<int>((xb >> 32) & 0xffff), static_cast<int>((rows - 1) * p.ld_q + p.last_chunk + 16), 0x00027000};
-  i32x4 wr = {static_cast<int>(wb), static_cast<int>((wb >> 32) & 0xffff), BN * p.kb * 64, 0x00027000};
+  i32x4 wr = {static_cast<int>(wb), static_cast<int>((wb >> 32) & 0xffff), 2 * kPadN * 64 * p.kb, 0x00027000};
 #pragma unroll
   for (int i = 0; i < 4; i++) { xr[i] = __builtin_amdgcn_readfirstlane(xr[i]); wr[i] = __builtin_amdgcn_readfirstlane(wr[i]); }
 
@@ -168,14 +201,18 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   auto load = [&](unsigned to, i32x4 rsrc, int voff, int soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
   };
-  auto issue = [&](int kt, int stage) {
+  auto issue = [&](int kt, int stage, int first, int last) {     // loads first .. last - 1 of this wave's for a stage
     const unsigned at = lds + stage * STAGE;
 #pragma unroll
-    for (int i = 0; i < X_PW; i++) load(at + (wave + NW * i) * 1024, xr, x_row[i] + min(kt * 128 + x_chunk[i], p.last_chunk), 0);
-#pragma unroll
-    for (int i = 0; i < W_PW; i++) {
-      const int j = wave + NW * i;                               // block j / 2 of 16 channels, half j % 2 of the 128 codes
-      load(at + X_BYTES + j * 1024, wr, lane * 16, ((j >> 1) * p.kb + kt * 2 + (j & 1)) * 1024);
+    for (int l = 0; l < LOADS; l++) {
+      if (l < first || l >= last) continue;
+      if (l < X_PW) {
+        load(at + (wave + NW * l) * 1024, xr, x_row[l] + min(kt * 128 + x_chunk[l], p.last_chunk), 0);
+      } else {
+        const int j = wave + NW * (l - X_PW), h = j / (BN / 16); // half h of the 128 codes, block j % (BN / 16) of 16 channels
+        const int b = min(n0 / 16 + j % (BN / 16), p.np / 16 - 1) - n0 / kPadN * 16;
+        load(at + X_BYTES + j * 1024, wr, lane * 16, ((((b >> 4) * p.kb + kt * 2 + h) << 4) + (b & 15)) * 1024);
+      }
     }
   };
 
@@ -185,43 +222,102 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
 #pragma unroll
     for (int j = 0; j < TJ; j++) acc[i][j] = i32x4{0, 0, 0, 0};
   const int steps = p.kb >> 1;
+  const int xoff = (wm * (BM / WM) + (lane & 15)) * 128, xslot = (lane >> 4) ^ ((lane >> 1) & 7);
+  const int woff = X_BYTES + wn * (BN / WN / 16) * 1024 + lane * 16;
+  struct Fragments { i32x4 w[TJ], x[TI]; } half0, half1;         // 64 codes each
+  auto fetch_w = [&](int stage, int h, int j, Fragments *f) {
+    f->w[j] = *reinterpret_cast<const i32x4 *>(smem + stage * STAGE + woff + (h * (BN / 16) + j) * 1024);
+  };
+  auto fetch_x = [&](int stage, int h, int i, Fragments *f) {
+    f->x[i] = *reinterpret_cast<const i32x4 *>(smem + stage * STAGE + xoff + i * 2048 + ((xslot ^ (h * 4)) * 16));
+  };
+  // One half of a stage is multiplied while the next is read and a later stage is asked for: a few of each at a time, since a
+  // wave issues in order and both the LDS and the load path would hold it up, the matrix unit idle, if asked all at once.
+  // FETCH: the fragments of half `h` of `stage` go to `next`; LOAD: stage `kt` is loaded into `slot`.
+  auto half = [&](const Fragments &now, Fragments *next, int stage, int h, auto fetch, auto load_too, int kt, int slot) {
 #pragma unroll
-  for (int s = 0; s < NST - 1; s++)
-    if (s < steps) issue(s, s);
-  const int xoff = (lane & 15) * 128, xslot = (lane >> 4) ^ ((lane >> 1) & 7);
-  int stage = 0;
-  for (int kt = 0; kt < steps; kt++) {
-    if (NST > 2 && kt + NST - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * LOADS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();                                // this stage is there, and the one before has been read by all
-    asm volatile("" ::: "memory");
-    if (kt + NST - 1 < steps) issue(kt + NST - 1, stage == 0 ? NST - 1 : stage - 1);
-    const unsigned char *xs = smem + stage * STAGE + wm * (BM / WM) * 128 + xoff;
-    const unsigned char *ws = smem + stage * STAGE + X_BYTES + wn * (BN / WN / 16) * 2048 + lane * 16;
+    for (int i = 0; i < TI; i++) {
+      if constexpr (decltype(fetch)::value) {
+        fetch_x(stage, h, i, next);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      i32x4 a[TJ], b[TI];
+        for (int j = i * TJ / TI; j < (i + 1) * TJ / TI; j++) fetch_w(stage, h, j, next);
+      }
 #pragma unroll
-      for (int j = 0; j < TJ; j++) a[j] = *reinterpret_cast<const i32x4 *>(ws + (j * 2 + h) * 1024);
-#pragma unroll
-      for (int i = 0; i < TI; i++) b[i] = *reinterpret_cast<const i32x4 *>(xs + i * 2048 + ((xslot ^ (h * 4)) * 16));
-#pragma unroll
-      for (int i = 0; i < TI; i++)
-#pragma unroll
-        for (int j = 0; j < TJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], b[i], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < TJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.w[j], now.x[i], acc[i][j], 0, 0, 0);
+      if constexpr (decltype(load_too)::value) issue(kt, slot, i * LOADS / TI, (i + 1) * LOADS / TI);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  typedef std::integral_constant<bool, true> Yes;
+  typedef std::integral_constant<bool, false> No;
+#pragma unroll
+  for (int t = 0; t < NST; t++)
+    if (t < steps) issue(t, t, 0, LOADS);
+  WaitBut<LOADS, NST - 1>(min(NST, steps) - 1);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < TJ; j++) fetch_w(0, 0, j, &half0);
+#pragma unroll
+  for (int i = 0; i < TI; i++) fetch_x(0, 0, i, &half0);
+  int stage = 0, kt = 0;
+  auto next_stage = [&]() {
+    __builtin_amdgcn_s_barrier();                                // the next stage is there, and this one has been read by all
+    asm volatile("" ::: "memory");
     stage = stage + 1 == NST ? 0 : stage + 1;
+  };
+  for (; kt + NST < steps; kt++) {
+    half(half0, &half1, stage, 1, Yes(), No(), 0, 0);
+    WaitBut<LOADS, NST - 2>(NST - 2);
+    const int slot = stage;
+    next_stage();
+    half(half1, &half0, stage, 0, Yes(), Yes(), kt + NST, slot);
+  }
+  for (; kt + 1 < steps; kt++) {
+    half(half0, &half1, stage, 1, Yes(), No(), 0, 0);
+    WaitBut<LOADS, NST - 2>(min(NST - 2, steps - 2 - kt));
+    next_stage();
+    half(half1, &half0, stage, 0, Yes(), No(), 0, 0);
+  }
+  half(half0, &half1, stage, 1, Yes(), No(), 0, 0);
+  half(half1, &half0, stage, 0, No(), No(), 0, 0);
+
+  // The output leaves in whole cache lines: a lane holds 4 channels of one row, so that stores from the registers would touch
+  // 16 rows with 8 to 16 bytes each.  Every wave turns its tile through a corner of the LDS of its own, 16 rows at a time.
+  constexpr int VE = 16 / static_cast<int>(sizeof(TO)), COLS = BN / WN, PITCH = COLS * static_cast<int>(sizeof(TO)) + 16, LPR = COLS / VE, RPI = 64 / LPR;
+  static_assert(NW * 16 * PITCH <= NST * STAGE && LPR <= 64 && RPI <= 16, "epilogue");
+  typedef TO OV __attribute__((ext_vector_type(VE)));
+  typedef TO OV4 __attribute__((ext_vector_type(4)));
+  __syncthreads();
+  unsigned char *mine = smem + wave * 16 * PITCH;
+  const int nw = n0 + wn * COLS, n4 = nw + (lane >> 4) * 4;
+  f32x4 w_scale[TJ], bias[TJ];
+#pragma unroll
+  for (int j = 0; j < TJ; j++) {
+    const int n = min(n4 + j * 16, p.np - 4);
+    w_scale[j] = *reinterpret_cast<const f32x4 *>(p.col + n);
+    bias[j] = *reinterpret_cast<const f32x4 *>(p.col + p.np + n);
   }
 #pragma unroll
   for (int i = 0; i < TI; i++) {
-    const int m = m0 + wm * (BM / WM) + i * 16 + (lane & 15);
-    if (m >= p.rows) continue;
-    const float scale = p.scale[m];
+    const int mi = m0 + wm * (BM / WM) + i * 16;
+    const float scale = p.scale[min(mi + (lane & 15), p.rows - 1)];
 #pragma unroll
     for (int j = 0; j < TJ; j++) {
-      const int n = n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4;
-      if (n < p.n) FinishFour<TO>(p, acc[i][j], scale, m, n);
+      const f32x4 z = Finish(p, acc[i][j], scale, w_scale[j], bias[j], min(n4 + j * 16, p.np - 4));
+      StoreAny(mine + (lane & 15) * PITCH + ((lane >> 4) * 4 + j * 16) * sizeof(TO), __builtin_convertvector(z, OV4));
     }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += RPI) {                       // LPR lanes to a row, RPI rows at once
+      const int r = r0 + lane / LPR, n = nw + lane % LPR * VE;
+      if ((64 % LPR == 0 || (lane < RPI * LPR && r < 16)) && mi + r < p.rows && n < p.n) {
+        OV v;
+        __builtin_memcpy(&v, mine + r * PITCH + lane % LPR * 16, 16);
+        StoreRow<VE, TO>(p, mi + r, n, v);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -230,8 +326,9 @@ __global__ __launch_bounds__(256) void PackKernel(const int8_t *w, int64_t ld, i
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= chunks) return;
   const int lane = static_cast<int>(i & 63);
-  const int64_t block = i >> 6;
-  const int row = static_cast<int>(block / kb) * 16 + (lane & 15), at = static_cast<int>(block % kb) * 64 + (lane >> 4) * 16;
+  const int64_t block = i >> 6, step = block >> 4;               // 16 blocks of 16 channels to a step of 64 codes
+  const int row = static_cast<int>(step / kb) * kPadN + static_cast<int>(block & 15) * 16 + (lane & 15);
+  const int at = static_cast<int>(step % kb) * 64 + (lane >> 4) * 16;
   int8_t v[16];
 #pragma unroll
   for (int j = 0; j < 16; j++) v[j] = row < n && at + j < k ? w[row * ld + at + j] : 0;
@@ -249,18 +346,51 @@ __global__ __launch_bounds__(256) void ColumnsKernel(const float *w_scale, const
   to[3 * np + i] = in && add ? add[i] : 0.0f;
 }
 
+template <int TI, int TJ, typename TO>
+void LaunchSplit(AffineArgs p, hipStream_t st) {
+  p.tiles_m = CeilDiv(p.rows, TI * 16); p.tiles_n = CeilDiv(p.n, TJ * 16);
+  hipLaunchKernelGGL((SplitKernel<TI, TJ, TO>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
+}
+
+template <int BM, int BN, int WM, int WN, int NST, typename TO>
+void LaunchTile(AffineArgs p, hipStream_t st) {
+  p.tiles_m = CeilDiv(p.rows, BM); p.tiles_n = CeilDiv(p.n, BN);
+  hipLaunchKernelGGL((TileKernel<BM, BN, WM, WN, NST, TO>), dim3(p.tiles_m * p.tiles_n), dim3(WM * WN * 64), 0, st, p);
+}
+
+// Which kernel.  A call takes about  2 us + c (s step + fixed),  c = tiles per CU, s = steps of 128 codes, with the two constants
+// of each kernel measured on MI355X; the cheapest is taken.  What the kernels are for, each against its neighbour (us):
+//   32 x 32 split    40 x 1536 x 1536   4.0   (64 x 64  5.0)     64 x 4096 x 4096  6.9 (8.9)    24 x 6000 x 1536  3.7 (16 x 16 split 4.8)
+//   64 x 64, 4 st.   256 x 4096 x 4096  9.5   (64 x 128 12.1)    1000 x 768 x 768  4.0 (4.9)
+//   64 x 128, 3 st.  512 x 4096 x 4096  13.3  (64 x 64 15.7)
+//   128 x 192, 3 st. 1999 x 2328 x 1537 14.3  (64 x 128 16.6, 2 stages 16.4): one tile per CU, so that it can have all the LDS
+//   128 x 192, 2 st. 12000 x 1536 x 1536 34   (256 x 256 45.5, 3 stages 37.7): two tiles per CU cover each other's waits
+//   256 x 256, 2 st. 4096 x 4096 x 4096 55.9  (128 x 192 68.9)   16384 x 8192 x 8192  847 (943)
+struct Cost { int bm, bn; double step, fixed; };
+constexpr int kCus = 256;
+constexpr Cost kSplit32 = {32, 32, 0.135, 0.3}, kTile64 = {64, 64, 0.19, 0.9}, kTile64x128 = {64, 128, 0.29, 1.2}, kTile128x192Alone = {128, 192, 0.40, 5.0},
+               kTile128x192 = {128, 192, 0.62, 2.8}, kTile256 = {256, 256, 1.42, 8.0};
+
 template <typename TO>
-int Propagate(const AffineArgs &a, hipStream_t st) {
-  AffineArgs p = a;
-  if (p.rows <= 64) {
-    const dim3 grid(CeilDiv(p.n, 16));
-    if (p.rows <= 16) hipLaunchKernelGGL((FewRowsKernel<1, TO>), grid, dim3(512), 0, st, p);
-    else if (p.rows <= 32) hipLaunchKernelGGL((FewRowsKernel<2, TO>), grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((FewRowsKernel<4, TO>), grid, dim3(512), 0, st, p);
-  } else {
-    p.tiles_m = CeilDiv(p.rows, 128); p.tiles_n = CeilDiv(p.n, 128);
-    hipLaunchKernelGGL((TileKernel<128, 128, 2, 2, 2, TO>), dim3(p.tiles_m * p.tiles_n), dim3(256), 0, st, p);
-  }
+int Propagate(const AffineArgs &p, hipStream_t st) {
+  const double steps = p.kb / 2;
+  auto per_cu = [&](const Cost &c) { return CeilDiv(static_cast<int64_t>(CeilDiv(p.rows, c.bm)) * CeilDiv(p.n, c.bn), kCus); };
+  auto cost = [&](const Cost &c) { return per_cu(c) * (steps * c.step + c.fixed); };
+  int which = 0;
+  double least = cost(kSplit32);
+  auto better = [&](int k, const Cost &c) { const double v = cost(c); if (v < least) { least = v; which = k; } };
+  better(1, kTile64);
+  better(2, kTile64x128);
+  if (per_cu(kTile128x192Alone) == 1) better(3, kTile128x192Alone);
+  better(4, kTile128x192);
+  better(5, kTile256);
+  if (p.rows <= 16) LaunchSplit<1, 1, TO>(p, st);
+  else if (which == 0) LaunchSplit<2, 2, TO>(p, st);
+  else if (which == 1) LaunchTile<64, 64, 4, 2, 4, TO>(p, st);
+  else if (which == 2) LaunchTile<64, 128, 2, 4, 3, TO>(p, st);
+  else if (which == 3) LaunchTile<128, 192, 2, 4, 3, TO>(p, st);
+  else if (which == 4) LaunchTile<128, 192, 2, 4, 2, TO>(p, st);
+  else LaunchTile<256, 256, 2, 4, 2, TO>(p, st);
   KAMD_HIP(hipGetLastError());
   return KAMD_OK;
 }

@@ -40,45 +40,54 @@ def _fail():
     raise KamdError(_L.kamd_last_error().decode())
 
 
-def _matrix(t, what, dtype=None, like=None):
-    """leading dimension of a matrix on the device; raises unless it is one"""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _matrix(t, what, dtype=None, shape=None, dev=-1):
+    """leading dimension of a matrix on the device (of this type, shape and device, where given); raises unless it is one.
+    Small calls are bound by what happens here and at the launch: a few attribute reads per tensor."""
+    if not getattr(t, "is_cuda", False):
         raise KamdError("%s: a tensor on the GPU is expected" % what)
     if t.dim() != 2:
         raise KamdError("%s: a matrix is expected, got shape %s" % (what, tuple(t.shape)))
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise KamdError("%s: %s expected, got %s" % (what, dtype, t.dtype))
-    if like is not None and t.device != like.device:
-        raise KamdError("%s: on %s, the other arguments on %s" % (what, t.device, like.device))
-    rows, cols = t.shape
+    if shape is not None and t.shape != shape:
+        raise KamdError("%s: shape %s expected, got %s" % (what, tuple(shape), tuple(t.shape)))
+    if dev >= 0 and t.get_device() != dev:
+        raise KamdError("%s: on %s, the other arguments on cuda:%d" % (what, t.device, dev))
     ld, step = t.stride()
+    rows, cols = t.shape
     if step != 1 and cols > 1:
         raise KamdError("%s: the values of a row have to be contiguous (strides %s)" % (what, (ld, step)))
-    return ld if rows > 1 else max(ld, cols)
+    return ld if rows > 1 or ld > cols else cols
 
 
-def _vector(t, n, what, like):
-    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
-        raise KamdError("%s: a float32 vector of %d on %s is expected" % (what, n, like.device))
-    if not t.is_contiguous():
-        raise KamdError("%s: has to be contiguous" % what)
+def _empty_as(x):
+    """[rows x dim] like x, without gaps between the rows"""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _vector(t, n, what, dev):
+    if not getattr(t, "is_cuda", False) or t.dtype is not torch.float32 or t.dim() != 1 or len(t) != n or t.get_device() != dev or not t.is_contiguous():
+        raise KamdError("%s: a contiguous float32 vector of %d on cuda:%d is expected" % (what, n, dev))
     return t.data_ptr()
 
 
-def _type(t, what):
-    code = _TYPES.get(t.dtype)
+def _type(dtype, what):
+    code = _TYPES.get(dtype)
     if code is None:
-        raise KamdError("%s: float32, bfloat16 or float16 expected, got %s" % (what, t.dtype))
+        raise KamdError("%s: float32, bfloat16 or float16 expected, got %s" % (what, dtype))
     return code
 
 
-def _call(device, fn, *args):
-    """fn(*args, stream) with `device` as the current one"""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+_current_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _call(dev, fn, *args):
+    """fn(*args, stream) with device `dev` as the current one"""
+    if dev == _current_device():
+        rc = fn(*args, _stream(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
     if rc < 0:
         _fail()
 
@@ -88,27 +97,35 @@ def empty_codes(rows, dim, device):
     return torch.empty((rows, (dim + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :dim]
 
 
-def _norm(x, gain, eps, residual, sum_out, out, ld_out, out_type, scale):
-    L = _library()
+def _norm(x, gain, eps, residual, sum_out, out, scale):
+    """the call behind rms_norm (scale None) and rms_norm_int8; out = the output and its leading dimension, or None"""
+    L = _L or _library()
     ld_x = _matrix(x, "x")
-    rows, dim = x.shape
-    code = _type(x, "x")
-    ld_r = ld_s = 0
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    rows, dim = shape
+    code = _type(dtype, "x")
+    r = h = g = None
+    ld_r = ld_h = 0
     if residual is not None:
-        ld_r = _matrix(residual, "residual", x.dtype, x)
+        ld_r = _matrix(residual, "residual", dtype, shape, dev)
+        r = residual.data_ptr()
         if sum_out is None:
-            sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            sum_out = _empty_as(x)
+            ld_h = dim
     if sum_out is not None:
-        ld_s = _matrix(sum_out, "sum_out", x.dtype, x)
-    for t, what in ((residual, "residual"), (sum_out, "sum_out")):
-        if t is not None and t.shape != x.shape:
-            raise KamdError("%s: shape %s expected, got %s" % (what, tuple(x.shape), tuple(t.shape)))
-    g = None if gain is None else _vector(gain, dim, "gain", x)
+        if not ld_h:
+            ld_h = _matrix(sum_out, "sum_out", dtype, shape, dev)
+        h = sum_out.data_ptr()
+    if gain is not None:
+        g = _vector(gain, dim, "gain", dev)
+    if out is None:
+        y, ld_y = _empty_as(x), dim
+    else:
+        y, ld_y = out
     if rows:
-        _call(x.device, L.kamd_rms_norm_device, x.data_ptr(), ld_x, None if residual is None else residual.data_ptr(), ld_r, code, g, eps, rows, dim,
-              None if sum_out is None else sum_out.data_ptr(), ld_s, out.data_ptr(), ld_out, code if out_type is None else out_type,
-              None if scale is None else scale.data_ptr())
-    return sum_out
+        _call(dev, L.kamd_rms_norm_device, x.data_ptr(), ld_x, r, ld_r, code, g, eps, rows, dim, h, ld_h, y.data_ptr(), ld_y,
+              code if scale is None else _I8, None if scale is None else scale.data_ptr())
+    return y, sum_out
 
 
 def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
@@ -117,47 +134,46 @@ def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
     x: [rows, dim] float32 / bfloat16 / float16, rows any stride apart; residual: the same shape and type; gain: float32 [dim].
     NormalizeComponent is gain = target_rms, eps = 2^-66.  sum_out (h) and out (y) may be given; sum_out may be x or residual,
     out any of the three."""
-    ld_x = _matrix(x, "x")
+    if out is not None:
+        _matrix(x, "x")
+        out = out, _matrix(out, "out", x.dtype, x.shape, x.get_device())
+    y, h = _norm(x, gain, eps, residual, sum_out, out, None)
+    return y if h is None else (y, h)
+
+
+def _codes_out(out, rows, dim, x):
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ld_out = _matrix(out, "out", x.dtype, x)
-    if out.shape != x.shape:
-        raise KamdError("out: shape %s expected, got %s" % (tuple(x.shape), tuple(out.shape)))
-    h = _norm(x, gain, eps, residual, sum_out, out, ld_out, None, None)
-    return out if h is None else (out, h)
+        q = empty_codes(rows, dim, x.device)
+        return q, torch.empty(rows, dtype=torch.float32, device=x.device), q.stride(0)
+    q, scale = out
+    ld_q = _matrix(q, "codes", torch.int8, (rows, dim), x.get_device())
+    _vector(scale, rows, "scale", x.get_device())
+    return q, scale, ld_q
 
 
 def rms_norm_int8(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
     """rms_norm with y as 8-bit rows -> (codes, scale), or (codes, scale, h) with a residual.  out = (codes, scale) may be given."""
     _matrix(x, "x")
     q, scale, ld_q = _codes_out(out, x.shape[0], x.shape[1], x)
-    h = _norm(x, gain, eps, residual, sum_out, q, ld_q, _I8, scale)
+    _, h = _norm(x, gain, eps, residual, sum_out, (q, ld_q), scale)
     return (q, scale) if h is None else (q, scale, h)
-
-
-def _codes_out(out, rows, dim, like):
-    q, scale = out if out is not None else (empty_codes(rows, dim, like.device), torch.empty(rows, dtype=torch.float32, device=like.device))
-    ld_q = _matrix(q, "codes", torch.int8, like)
-    if tuple(q.shape) != (rows, dim):
-        raise KamdError("codes: shape %s expected, got %s" % ((rows, dim), tuple(q.shape)))
-    _vector(scale, rows, "scale", like)
-    return q, scale, ld_q
 
 
 def quantize_rows(x, offsets=(0,), out=None):
     """8-bit rows of a (spliced) matrix -> (codes, scale): row j codes Append_i x[j + offsets[i] - min(offsets)], so that
     x.rows - (max - min) rows come back (kamd_quantize_rows_device; the input of a layer with these time offsets)."""
-    L = _library()
+    L = _L or _library()
     ld_x = _matrix(x, "x")
-    code = _type(x, "x")
-    offsets = [int(o) for o in offsets]
-    if not 1 <= len(offsets) <= abi.KAMD_MAX_OFFSETS:
+    in_rows, dim = x.shape
+    code = _type(x.dtype, "x")
+    n = len(offsets)
+    if not 1 <= n <= abi.KAMD_MAX_OFFSETS:
         raise KamdError("offsets: between 1 and %d of them expected" % abi.KAMD_MAX_OFFSETS)
-    rows = max(0, x.shape[0] - (max(offsets) - min(offsets)))
-    q, scale, ld_q = _codes_out(out, rows, x.shape[1] * len(offsets), x)
+    rows = max(0, in_rows - (max(offsets) - min(offsets)))
+    q, scale, ld_q = _codes_out(out, rows, dim * n, x)
     if rows:
-        _call(x.device, L.kamd_quantize_rows_device, x.data_ptr(), ld_x, code, x.shape[0], x.shape[1], (C.c_int32 * len(offsets))(*offsets), len(offsets),
-              q.data_ptr(), ld_q, scale.data_ptr())
+        _call(x.get_device(), L.kamd_quantize_rows_device, x.data_ptr(), ld_x, code, in_rows, dim, (C.c_int32 * n)(*offsets), n, q.data_ptr(), ld_q,
+              scale.data_ptr())
     return q, scale
 
 
@@ -171,7 +187,8 @@ class AffineInt8:
         L = _library()
         ld = _matrix(weight, "weight", torch.int8)
         n, k = weight.shape
-        vectors = [None if v is None else _vector(v, n, what, weight) for v, what in
+        dev = weight.get_device()
+        vectors = [None if v is None else _vector(v, n, what, dev) for v, what in
                    ((weight_scale, "weight_scale"), (bias, "bias"), (mul, "mul"), (add, "add"))]
         self.device, self.offsets = weight.device, (0,)
         with torch.cuda.device(weight.device):
@@ -199,7 +216,7 @@ class AffineInt8:
         self.in_dim, self.out_dim = _L.kamd_component_i8_input_dim(handle), _L.kamd_component_i8_output_dim(handle)
 
     def __del__(self):
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and _L is not None:
             _L.kamd_component_i8_destroy(self._h)
             self._h = None
 
@@ -211,22 +228,24 @@ class AffineInt8:
         """codes [rows, in_dim] and scales [rows] -> [rows, out_dim] of `dtype`"""
         ld_q = _matrix(q, "codes", torch.int8)
         rows, k = q.shape
-        if k != self.in_dim or q.device != self.device:
+        dev = q.get_device()
+        if k != self.in_dim or dev != self.device.index:
             raise KamdError("codes: [rows, %d] on %s expected, got %s on %s" % (self.in_dim, self.device, tuple(q.shape), q.device))
         if rows <= 1:
             ld_q = (ld_q + 15) // 16 * 16
-        if ld_q % 16 or q.data_ptr() % 16:
+        at = q.data_ptr()
+        if ld_q % 16 or at % 16:
             raise KamdError("codes: rows begin on multiples of 16 bytes (int8.empty_codes has the layout)")
         if k % 16 and q.untyped_storage().nbytes() - q.storage_offset() < (rows - 1) * ld_q + (k + 15) // 16 * 16:
             raise KamdError("codes: the last row ends inside a block of 16 bytes that is not the tensor's own")
-        s = _vector(scale, rows, "scale", q)
+        s = _vector(scale, rows, "scale", dev)
+        code = _type(dtype, "dtype")
         if out is None:
-            out = torch.empty((rows, self.out_dim), dtype=dtype, device=q.device)
-        ld_out = _matrix(out, "out", dtype, q)
-        if tuple(out.shape) != (rows, self.out_dim):
-            raise KamdError("out: shape %s expected, got %s" % ((rows, self.out_dim), tuple(out.shape)))
+            out, ld_out = torch.empty((rows, self.out_dim), dtype=dtype, device=q.device), self.out_dim
+        else:
+            ld_out = _matrix(out, "out", dtype, (rows, self.out_dim), dev)
         if rows:
-            _call(q.device, _L.kamd_component_i8_propagate, self._h, q.data_ptr(), ld_q, s, rows, out.data_ptr(), ld_out, _type(out, "out"))
+            _call(dev, _L.kamd_component_i8_propagate, self._h, at, ld_q, s, rows, out.data_ptr(), ld_out, code)
         return out
 
     def Propagate(self, x, dtype=None):

@@ -250,6 +250,21 @@ def test_product_of_many_tiles(rows, k, n):
     both(rows, k, n, torch.float32, full=False)
 
 
+@pytest.mark.parametrize("rows, k, n", [(17, 130, 300), (100, 1000, 100), (500, 4000, 1000), (1000, 1500, 2000), (2000, 1537, 2328), (7000, 500, 1500),
+                                        (3900, 1030, 4000), (8100, 700, 8000)])
+def test_product_in_each_of_its_kernels(rows, k, n):
+    """sizes at which the cost rule takes the split kernel, the 64 x 64, 64 x 128, 128 x 192 (one and two to a CU) and 256 x 256
+    tiles, with rows, channels and codes that end inside a tile; the exact sums come from 64-bit products on the device"""
+    w, ws, bias, mul, add = layer_of(k, n, 51, True)
+    q, scale = codes(rows, k, 52), torch.rand(rows)
+    d = [t.cuda() for t in (q, scale, w, ws, bias, mul, add)]
+    layer = int8.AffineInt8(d[2], d[3], d[4], True, d[5], d[6])
+    for dtype in TYPES:
+        y = layer.propagate(on_device(q, 16), d[1], dtype)
+        want, bound = product64(d[0], d[1], d[2], d[3], d[4], True, d[5], d[6])
+        check_product(y, want.cpu(), bound.cpu(), dtype)
+
+
 def test_product_at_the_limits_of_its_sum():
     """the longest row of the largest codes: a sum of 2^31 - 16384 and one of its negative"""
     k = 131071
