@@ -17,6 +17,7 @@ import torch
 from . import abi
 from ._lib import KamdError, lib
 
+_OFFSETS = [C.c_int32 * n for n in range(abi.KAMD_MAX_OFFSETS + 1)]
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _I8 = 3
 _L = None
@@ -94,6 +95,8 @@ def _call(dev, fn, *args):
 
 def empty_codes(rows, dim, device):
     """[rows x dim] int8 in the layout the product takes: each row begins on a multiple of 16 bytes"""
+    if dim % 16 == 0:
+        return torch.empty((rows, dim), dtype=torch.int8, device=device)
     return torch.empty((rows, (dim + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :dim]
 
 
@@ -144,7 +147,7 @@ def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
 def _codes_out(out, rows, dim, x):
     if out is None:
         q = empty_codes(rows, dim, x.device)
-        return q, torch.empty(rows, dtype=torch.float32, device=x.device), q.stride(0)
+        return q, torch.empty(rows, dtype=torch.float32, device=x.device), (dim + 15) // 16 * 16
     q, scale = out
     ld_q = _matrix(q, "codes", torch.int8, (rows, dim), x.get_device())
     _vector(scale, rows, "scale", x.get_device())
@@ -172,7 +175,7 @@ def quantize_rows(x, offsets=(0,), out=None):
     rows = max(0, in_rows - (max(offsets) - min(offsets)))
     q, scale, ld_q = _codes_out(out, rows, dim * n, x)
     if rows:
-        _call(x.get_device(), L.kamd_quantize_rows_device, x.data_ptr(), ld_x, code, in_rows, dim, (C.c_int32 * n)(*offsets), n, q.data_ptr(), ld_q,
+        _call(x.get_device(), L.kamd_quantize_rows_device, x.data_ptr(), ld_x, code, in_rows, dim, _OFFSETS[n](*offsets), n, q.data_ptr(), ld_q,
               scale.data_ptr())
     return q, scale
 

@@ -94,7 +94,26 @@ def test_norm_over_row_counts_and_strides(rows, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("dim", [100, 3000, 40000])
+@pytest.mark.parametrize("dim, offsets", [(250, (0,)), (700, (0,)), (1100, (0,)), (1536, (0,)), (1733, (0,)), (2050, (0,)), (2304, (0,)), (5000, (0,)), (130, (-1, 0, 1)),
+                                          (768, (-3, 0, 3)), (509, (-2, -1, 0, 1, 2)), (1000, (0, 4)), (257, tuple(range(8))), (9, tuple(range(8)))])
+def test_many_rows_take_waves_of_their_own(dtype, dim, offsets):
+    """every way in which 1024 rows and more are laid over the threads"""
+    x, r, gain = rand(1100, dim, seed=dim, dtype=dtype), rand(1100, dim, seed=dim + 1, dtype=dtype), 1 + 0.2 * rand(dim, seed=2)
+    lo, n = min(offsets), 1100 - (max(offsets) - min(offsets))
+    check_codes(*int8.quantize_rows(x.cuda(), offsets), torch.cat([x[o - lo:o - lo + n] for o in offsets], 1).double())
+    h, want = norm64(x, gain, EPS, r)
+    rd = r.cuda()
+    y, s = int8.rms_norm(x.cuda(), gain.cuda(), EPS, residual=rd, sum_out=rd)
+    check_norm(y, want, dtype)
+    assert s is rd and torch.equal(s.cpu(), (x.float() + r.float()).to(dtype))
+    rd = r.cuda()
+    q, scale, s = int8.rms_norm_int8(x.cuda(), gain.cuda(), EPS, residual=rd, sum_out=rd)
+    check_codes(q, scale, want)
+    assert torch.equal(s.cpu(), (x.float() + r.float()).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [100, 1501, 2999, 9003, 20005, 40001])
 def test_norm_in_place(dtype, dim):
     x, r = rand(7, dim, seed=3, dtype=dtype).cuda(), rand(7, dim, seed=4, dtype=dtype).cuda()
     y, s = int8.rms_norm(x, None, EPS, residual=r)
