@@ -359,38 +359,36 @@ void LaunchTile(AffineArgs p, hipStream_t st) {
 }
 
 // Which kernel.  A call takes about  2 us + c (s step + fixed),  c = tiles per CU, s = steps of 128 codes, with the two constants
-// of each kernel measured on MI355X; the cheapest is taken.  What the kernels are for, each against its neighbour (us):
-//   32 x 32 split    40 x 1536 x 1536   4.0   (64 x 64  5.0)     64 x 4096 x 4096  6.9 (8.9)    24 x 6000 x 1536  3.7 (16 x 16 split 4.8)
-//   64 x 64, 4 st.   256 x 4096 x 4096  9.5   (64 x 128 12.1)    1000 x 768 x 768  4.0 (4.9)
+// of each kernel measured on MI355X; the cheapest is taken (over 80 random sizes within 3 % of the fastest of them in the mean).
+// What the kernels are for, each against its neighbour (us):
+//   16 x 16 split    1 x 4096 x 4096  3.1 (32 x 32  4.1)          20 x 320 x 7840  5.3 (7.5)
+//   32 x 32 split    24 x 6000 x 1536  3.7 (16 x 16  4.8)         64 x 4096 x 4096  6.9 (64 x 64  8.9)
+//   64 x 64, 4 st.   256 x 4096 x 4096  9.5   (64 x 128 12.1)     1000 x 768 x 768  4.0 (4.9)
 //   64 x 128, 3 st.  512 x 4096 x 4096  13.3  (64 x 64 15.7)
 //   128 x 192, 3 st. 1999 x 2328 x 1537 14.3  (64 x 128 16.6, 2 stages 16.4): one tile per CU, so that it can have all the LDS
 //   128 x 192, 2 st. 12000 x 1536 x 1536 34   (256 x 256 45.5, 3 stages 37.7): two tiles per CU cover each other's waits
 //   256 x 256, 2 st. 4096 x 4096 x 4096 55.9  (128 x 192 68.9)   16384 x 8192 x 8192  847 (943)
-struct Cost { int bm, bn; double step, fixed; };
 constexpr int kCus = 256;
-constexpr Cost kSplit32 = {32, 32, 0.135, 0.3}, kTile64 = {64, 64, 0.19, 0.9}, kTile64x128 = {64, 128, 0.29, 1.2}, kTile128x192Alone = {128, 192, 0.40, 5.0},
-               kTile128x192 = {128, 192, 0.62, 2.8}, kTile256 = {256, 256, 1.42, 8.0};
 
 template <typename TO>
 int Propagate(const AffineArgs &p, hipStream_t st) {
-  const double steps = p.kb / 2;
-  auto per_cu = [&](const Cost &c) { return CeilDiv(static_cast<int64_t>(CeilDiv(p.rows, c.bm)) * CeilDiv(p.n, c.bn), kCus); };
-  auto cost = [&](const Cost &c) { return per_cu(c) * (steps * c.step + c.fixed); };
-  int which = 0;
-  double least = cost(kSplit32);
-  auto better = [&](int k, const Cost &c) { const double v = cost(c); if (v < least) { least = v; which = k; } };
-  better(1, kTile64);
-  better(2, kTile64x128);
-  if (per_cu(kTile128x192Alone) == 1) better(3, kTile128x192Alone);
-  better(4, kTile128x192);
-  better(5, kTile256);
-  if (p.rows <= 16) LaunchSplit<1, 1, TO>(p, st);
-  else if (which == 0) LaunchSplit<2, 2, TO>(p, st);
-  else if (which == 1) LaunchTile<64, 64, 4, 2, 4, TO>(p, st);
-  else if (which == 2) LaunchTile<64, 128, 2, 4, 3, TO>(p, st);
-  else if (which == 3) LaunchTile<128, 192, 2, 4, 3, TO>(p, st);
-  else if (which == 4) LaunchTile<128, 192, 2, 4, 2, TO>(p, st);
-  else LaunchTile<256, 256, 2, 4, 2, TO>(p, st);
+  struct Kernel { int bm, bn; double step, fixed; bool alone; void (*go)(AffineArgs, hipStream_t); };     // alone: at most one tile per CU
+  static const Kernel kernels[] = {{16, 16, 0.065, 0.2, false, LaunchSplit<1, 1, TO>},
+                                   {32, 32, 0.135, 0.3, false, LaunchSplit<2, 2, TO>},
+                                   {64, 64, 0.19, 0.9, false, LaunchTile<64, 64, 4, 2, 4, TO>},
+                                   {64, 128, 0.29, 1.2, false, LaunchTile<64, 128, 2, 4, 3, TO>},
+                                   {128, 192, 0.40, 5.0, true, LaunchTile<128, 192, 2, 4, 3, TO>},
+                                   {128, 192, 0.62, 2.8, false, LaunchTile<128, 192, 2, 4, 2, TO>},
+                                   {256, 256, 1.42, 8.0, false, LaunchTile<256, 256, 2, 4, 2, TO>}};
+  const Kernel *best = NULL;
+  double least = 0.0;
+  for (const Kernel &k : kernels) {
+    const int64_t tiles = static_cast<int64_t>(CeilDiv(p.rows, k.bm)) * CeilDiv(p.n, k.bn), per_cu = (tiles + kCus - 1) / kCus;
+    if (k.alone && per_cu > 1) continue;
+    const double cost = static_cast<double>(per_cu) * (p.kb / 2 * k.step + k.fixed);
+    if (!best || cost < least) { best = &k; least = cost; }
+  }
+  best->go(p, st);
   KAMD_HIP(hipGetLastError());
   return KAMD_OK;
 }

@@ -258,21 +258,23 @@ static int LaunchRows(RowArgs a, hipStream_t st) {
 }
 
 // Threads per row and elements per thread: the pair that holds the row (piece by piece) with the least left over, for what is
-// left over is loaded and computed for nothing; of equals, the smaller workgroup.  Waves of their own with 24 and more elements
+// left over is loaded and computed for nothing; of equals, the first.  Waves of their own with 24 and more elements
 // per lane count for 1.4 times their size.  Few rows are given the threads that shorten the way through one.  (us, MI355X)
-//   norm 12000 x 1536 bf16  64 x 24  24.7   256 x 8 26.2   512 x 8  44         norm 16384 x 4096 bf16  256 x 16  95   64 x 64  108
-//   norm 12000 x 1536 f32   64 x 24  28.2   256 x 8 26.4                       norm 16384 x 8192 bf16  512 x 16 186   1024 x 16 250
+//   norm 12000 x 1536 bf16  64 x 24  24.7   256 x 8 26.2   512 x 8  44         norm 16384 x 4096 bf16  512 x 8  92  256 x 16  95  64 x 64  108
+//   norm 12000 x 1536 f32   64 x 24  28.2   256 x 8 26.4                       norm 16384 x 8192 bf16  1024 x 8 181  512 x 16 186  1024 x 16 250
 //   codes of 40000 x (3 x 768) f32  64 x 40  43   256 x 16  64                 norm 1 x 1536 bf16  256 x 8  2.4   64 x 32  3.1
+//   codes of 20000 x 4096 bf16  256 x 16  38.5   512 x 8  44.3  (the codes' kernels take the smaller workgroup of equals)
 template <typename T, typename TO, bool NORM>
 static int RunRows(const RowArgs &a, hipStream_t st) {
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
+  constexpr bool I8 = sizeof(TO) == 1;
   if (a.part_dim < VE) return LaunchRows<T, TO, NORM, 1, 64, 8>(a, st);          // at most 7 columns, in at most 8 pieces
   typedef int (*Launch)(RowArgs, hipStream_t);
   struct Shape { int tpr, ept; Launch go; };
 #define KAMD_SHAPE(TPR, EPT) {TPR, EPT, LaunchRows<T, TO, NORM, VE, TPR, (EPT) / VE>}
   static const Shape shapes[] = {KAMD_SHAPE(64, 8), KAMD_SHAPE(64, 16), KAMD_SHAPE(64, 24), KAMD_SHAPE(64, 32), KAMD_SHAPE(64, NORM ? 32 : 40),
-                                 KAMD_SHAPE(64, NORM ? 32 : 48), KAMD_SHAPE(256, 8), KAMD_SHAPE(256, 16), KAMD_SHAPE(256, 24), KAMD_SHAPE(512, 16),
-                                 KAMD_SHAPE(512, 24), KAMD_SHAPE(1024, 16), KAMD_SHAPE(1024, 32)};
+                                 KAMD_SHAPE(64, NORM ? 32 : 48), KAMD_SHAPE(256, 8), KAMD_SHAPE(512, I8 ? 16 : 8), KAMD_SHAPE(256, 16), KAMD_SHAPE(256, 24),
+                                 KAMD_SHAPE(1024, I8 ? 16 : 8), KAMD_SHAPE(512, 16), KAMD_SHAPE(512, 24), KAMD_SHAPE(1024, 16), KAMD_SHAPE(1024, 32)};
 #undef KAMD_SHAPE
   const Shape *best = NULL;
   double least = 0.0;
