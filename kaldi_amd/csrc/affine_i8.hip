@@ -73,11 +73,14 @@ __device__ inline f32x4 Finish(const AffineArgs &p, i32x4 acc, float scale, f32x
 }
 
 // values n .. n + VE - 1 of a row of the output; those behind its end are dropped
-template <int VE, typename TO, typename V>
+template <int VE, bool STREAM, typename TO, typename V>
 __device__ inline void StoreRow(const AffineArgs &p, int m, int n, V v) {
+  typedef V Unaligned __attribute__((aligned(sizeof(TO))));
   TO *o = static_cast<TO *>(p.out) + m * p.ld_out + n;
-  if (n + VE <= p.n) StoreAny(o, v);
-  else
+  if (n + VE <= p.n) {
+    if (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<Unaligned *>(o));
+    else StoreAny(o, v);
+  } else
 #pragma unroll
     for (int j = 0; j < VE; j++)
       if (n + j < p.n) o[j] = v[j];
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(512) void SplitKernel(AffineArgs p) {
 #pragma unroll
     for (int v = 1; v < NW; v++) s += part[v][f][lane];
     const f32x4 z = Finish(p, s, p.scale[m], *reinterpret_cast<const f32x4 *>(p.col + n), *reinterpret_cast<const f32x4 *>(p.col + p.np + n), n);
-    StoreRow<4, TO>(p, m, n, __builtin_convertvector(z, OV));
+    StoreRow<4, false, TO>(p, m, n, __builtin_convertvector(z, OV));
   }
 }
 
@@ -167,7 +170,7 @@ __device__ inline void WaitBut(int stages) {
 // Many rows: BM rows x BN channels per workgroup of WM x WN waves, operands by DMA into a ring of NST stages of 128 codes in LDS.
 // The product is bound by the power that the matrix units draw: 16384 x 8192 x 8192 runs at 2.6 PFLOP/s with the clock at
 // 2.0 GHz of 2.4, against 3.5 when the operands stay in registers and 4.6 for the matrix instructions alone.
-template <int BM, int BN, int WM, int WN, int NST, typename TO>
+template <int BM, int BN, int WM, int WN, int NST, bool STREAM, typename TO>
 __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   constexpr int NW = WM * WN, TI = BM / WM / 16, TJ = BN / WN / 16;
   constexpr int X_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = X_BYTES + W_BYTES;
@@ -314,7 +317,7 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
       if ((64 % LPR == 0 || (lane < RPI * LPR && r < 16)) && mi + r < p.rows && n < p.n) {
         OV v;
         __builtin_memcpy(&v, mine + r * PITCH + lane % LPR * 16, 16);
-        StoreRow<VE, TO>(p, mi + r, n, v);
+        StoreRow<VE, STREAM, TO>(p, mi + r, n, v);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -352,10 +355,19 @@ void LaunchSplit(AffineArgs p, hipStream_t st) {
   hipLaunchKernelGGL((SplitKernel<TI, TJ, TO>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
 }
 
+// An output that the last-level cache (256 MB) could not keep for the next layer anyway goes past the caches, whose lines the
+// operands need more: 16384 x 8192 x 8192 to bf16 (268 MB) 791 us instead of 850, with the coding of its rows behind it 4.5 % less.
+// A smaller one does not: 12000 x 1536 x 1536 (37 MB) with the next layers behind it takes 2 % longer if it has to be fetched.
+constexpr int64_t kStreamBytes = 128 << 20;
+
 template <int BM, int BN, int WM, int WN, int NST, typename TO>
 void LaunchTile(AffineArgs p, hipStream_t st) {
   p.tiles_m = CeilDiv(p.rows, BM); p.tiles_n = CeilDiv(p.n, BN);
-  hipLaunchKernelGGL((TileKernel<BM, BN, WM, WN, NST, TO>), dim3(p.tiles_m * p.tiles_n), dim3(WM * WN * 64), 0, st, p);
+  const dim3 grid(p.tiles_m * p.tiles_n), block(WM * WN * 64);
+  if (static_cast<int64_t>(p.rows) * p.n * static_cast<int64_t>(sizeof(TO)) > kStreamBytes)
+    hipLaunchKernelGGL((TileKernel<BM, BN, WM, WN, NST, true, TO>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((TileKernel<BM, BN, WM, WN, NST, false, TO>), grid, block, 0, st, p);
 }
 
 // Which kernel.  A call takes about  2 us + c (s step + fixed),  c = tiles per CU, s = steps of 128 codes, with the two constants
@@ -367,7 +379,7 @@ void LaunchTile(AffineArgs p, hipStream_t st) {
 //   64 x 128, 3 st.  512 x 4096 x 4096  13.3  (64 x 64 15.7)
 //   128 x 192, 3 st. 1999 x 2328 x 1537 14.3  (64 x 128 16.6, 2 stages 16.4): one tile per CU, so that it can have all the LDS
 //   128 x 192, 2 st. 12000 x 1536 x 1536 34   (256 x 256 45.5, 3 stages 37.7): two tiles per CU cover each other's waits
-//   256 x 256, 2 st. 4096 x 4096 x 4096 55.9  (128 x 192 68.9)   16384 x 8192 x 8192  847 (943)
+//   256 x 256, 2 st. 4096 x 4096 x 4096 55.9  (128 x 192 68.9)   16384 x 8192 x 8192  791 (921)
 constexpr int kCus = 256;
 
 template <typename TO>

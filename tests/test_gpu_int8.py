@@ -284,6 +284,18 @@ def test_product_in_each_of_its_kernels(rows, k, n):
         check_product(y, want.cpu(), bound.cpu(), dtype)
 
 
+def test_an_output_larger_than_the_caches():
+    """over 128 MB: stored past the caches, with rows, channels and the leading dimension off every boundary"""
+    for rows, n, dtype in ((9001, 7777, torch.bfloat16), (300, 120001, torch.float32)):
+        w, ws, bias, _, _ = layer_of(40, n, 53, True)
+        q, scale = codes(rows, 40, 54), torch.rand(rows)
+        out = torch.full((rows + 1, n + 3), 7.0, dtype=dtype, device="cuda")
+        y = int8.AffineInt8(w.cuda(), ws.cuda(), bias.cuda()).propagate(on_device(q), scale.cuda(), dtype, out=out[:rows, 1:n + 1])
+        at = torch.cat([torch.arange(0, rows, 97), torch.tensor([rows - 1])])
+        check_product(y[at], *product64(q[at], scale[at], w, ws, bias, False, None, None), dtype)
+        assert bool((out[rows] == 7.0).all()) and bool((out[:, 0] == 7.0).all()) and bool((out[:, n + 1:] == 7.0).all())
+
+
 def test_product_at_the_limits_of_its_sum():
     """the longest row of the largest codes: a sum of 2^31 - 16384 and one of its negative"""
     k = 131071
