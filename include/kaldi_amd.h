@@ -262,7 +262,7 @@ enum { KAMD_F32 = 0, KAMD_BF16 = 1, KAMD_F16 = 2, KAMD_I8 = 3 };
  * gain of a pre-norm layer, row by row:
  *   h = x (+ residual),   sum = h,   out = h / sqrt(mean(h^2) + eps) * gain
  * d_residual, d_gain (float [dim]; NULL = ones; constant target_rms = --target-rms) and d_sum may be NULL.  NormalizeComponent's
- * floor is eps = 2^-66.  h is the 32-bit sum, also where d_sum rounds it to 16 bits.  out_type is `type`, or KAMD_I8: then out
+ * floor is eps = 2^-66.  h is the 32-bit sum, also where d_sum rounds it to 16 bits, and codes are made of the 32-bit h * gain.  out_type is `type`, or KAMD_I8: then out
  * holds codes in [-127, 127] and d_out_scale[row] their scale: out ~ code * scale, off by at most scale / 2; a row of zeros has
  * scale 0, one that holds an infinity or a NaN has scale NaN (and codes 0).  d_sum may be d_x or d_residual, and d_out (of the
  * input's type) any of the three, at the same leading dimension; other overlaps are not allowed. */

@@ -168,8 +168,9 @@ __device__ inline void WaitBut(int stages) {
 }
 
 // Many rows: BM rows x BN channels per workgroup of WM x WN waves, operands by DMA into a ring of NST stages of 128 codes in LDS.
-// The product is bound by the power that the matrix units draw: 16384 x 8192 x 8192 runs at 2.6 PFLOP/s with the clock at
-// 2.0 GHz of 2.4, against 3.5 when the operands stay in registers and 4.6 for the matrix instructions alone.
+// Large products are bound by the power that the matrix units draw: 16384 x 8192 x 8192 runs at 2.8 POP/s with the clock at
+// 1.9 GHz of 2.4 and the matrix units 66 % busy; the matrix instructions alone reach 4.6.  Sums of ~1536 codes keep them 45 % busy:
+// a tile's first loads and its output take a third of its time, which the other tile on the CU covers in part.
 template <int BM, int BN, int WM, int WN, int NST, bool STREAM, typename TO>
 __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   constexpr int NW = WM * WN, TI = BM / WM / 16, TJ = BN / WN / 16;
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   // one, chunks to last_chunk).
   const size_t xb = reinterpret_cast<size_t>(p.q + static_cast<int64_t>(m0) * p.ld_q), wb = reinterpret_cast<size_t>(p.w + static_cast<size_t>(n0 / kPadN) * p.kb * (kPadN * 64));
   i32x4 xr = {static_cast<int>(xb), static_cast<int>((xb >> 32) & 0xffff), static_cast<int>((rows - 1) * p.ld_q + p.last_chunk + 16), 0x00027000};
-  i32x4 wr = {static_cast<int>(wb), static_cast<int>((wb >> 32) & 0xffff), 2 * kPadN * 64 * p.kb, 0x00027000};
+  i32x4 wr = {static_cast<int>(wb), static_cast<int>((wb >> 32) & 0xffff), min(2, p.np / kPadN - n0 / kPadN) * kPadN * 64 * p.kb, 0x00027000};
 #pragma unroll
   for (int i = 0; i < 4; i++) { xr[i] = __builtin_amdgcn_readfirstlane(xr[i]); wr[i] = __builtin_amdgcn_readfirstlane(wr[i]); }
 
@@ -382,8 +383,18 @@ void LaunchTile(AffineArgs p, hipStream_t st) {
 //   256 x 256, 2 st. 4096 x 4096 x 4096 55.9  (128 x 192 68.9)   16384 x 8192 x 8192  791 (921)
 constexpr int kCus = 256;
 
+constexpr int kMaxRows = 1 << 22;         // per launch: the grid of the smallest tile stays within its limit
+
 template <typename TO>
-int Propagate(const AffineArgs &p, hipStream_t st) {
+int Propagate(AffineArgs p, hipStream_t st) {
+  if (p.rows > kMaxRows) {
+    AffineArgs rest = p;
+    rest.q += static_cast<int64_t>(kMaxRows) * p.ld_q; rest.scale += kMaxRows; rest.rows -= kMaxRows;
+    rest.out = static_cast<TO *>(p.out) + static_cast<int64_t>(kMaxRows) * p.ld_out;
+    p.rows = kMaxRows;
+    const int rc = Propagate<TO>(p, st);
+    return rc != KAMD_OK ? rc : Propagate<TO>(rest, st);
+  }
   struct Kernel { int bm, bn; double step, fixed; bool alone; void (*go)(AffineArgs, hipStream_t); };     // alone: at most one tile per CU
   static const Kernel kernels[] = {{16, 16, 0.065, 0.2, false, LaunchSplit<1, 1, TO>},
                                    {32, 32, 0.135, 0.3, false, LaunchSplit<2, 2, TO>},

@@ -8,7 +8,7 @@ call keeps anything for the next.  A layer in a row:
 
 8-bit rows are codes in [-127, 127] with one float scale per row: value ~ code * scale.  `kaldi_amd.int8` is the device-tensor
 form of kamd_rms_norm_device, kamd_quantize_rows_device and kamd_component_i8_* (include/kaldi_amd.h), which a C or C++ host
-calls on plain pointers.
+calls on plain pointers.  Inference only: there are no gradients.
 """
 import ctypes as C
 
@@ -54,6 +54,8 @@ def _matrix(t, what, dtype=None, shape=None, dev=-1):
         raise KamdError("%s: shape %s expected, got %s" % (what, tuple(shape), tuple(t.shape)))
     if dev >= 0 and t.get_device() != dev:
         raise KamdError("%s: on %s, the other arguments on cuda:%d" % (what, t.device, dev))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise KamdError("%s: has a gradient to keep track of, and these calls have none (torch.no_grad or detach)" % what)
     ld, step = t.stride()
     rows, cols = t.shape
     if step != 1 and cols > 1:

@@ -171,7 +171,7 @@ def test_rows_out_of_the_ordinary(dim):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim, offsets", [(40, (0,)), (40, (-1, 0, 1)), (43, (-3, 0, 3)), (768, (-3, 0, 3)), (768, (0, 3)), (5, (2,)), (7, (-1, 0, 1, 2, 5, -2, 3, 4)),
-                                          (1500, (3, -3)), (9001, (-1, 0, 1, 2)), (64, (5, 9))])
+                                          (1500, (3, -3)), (33, (1, 1, 0)), (9001, (-1, 0, 1, 2)), (64, (5, 9))])
 def test_quantize_splices(dtype, dim, offsets):
     x = rand(23, dim, seed=dim, dtype=dtype)
     q, scale = int8.quantize_rows(x.cuda(), offsets)
@@ -441,6 +441,46 @@ def test_captured_and_replayed_beside_eager_calls():
             int8.rms_norm(rand(5, 40, seed=seed).cuda())
 
 
+def test_captured_without_having_run():
+    """kernels whose first launch is in a capture"""
+    w, ws, bias, _, _ = layer_of(272, 1000, 61, True)
+    layer = int8.AffineInt8(w.cuda(), ws.cuda(), bias.cuda())
+    x = torch.zeros(610, 272, device="cuda", dtype=torch.float16)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        q, scale = int8.quantize_rows(x)
+        y = layer.propagate(q, scale, torch.float16)
+        n = int8.rms_norm(y)
+    for seed in range(3):
+        x.copy_(rand(610, 272, seed=seed, dtype=torch.float16))
+        g.replay()
+        torch.cuda.synchronize()
+        q2, scale2 = int8.quantize_rows(x)
+        y2 = layer.propagate(q2, scale2, torch.float16)
+        assert torch.equal(q, q2) and torch.equal(scale, scale2) and torch.equal(y, y2) and torch.equal(n, int8.rms_norm(y2))
+
+
+def test_more_rows_than_a_launch_takes():
+    rows = (1 << 22) + 77
+    w, ws, bias, _, _ = layer_of(16, 8, 62, True)
+    q = torch.randint(-127, 128, (rows, 16), dtype=torch.int8, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    scale = torch.rand(rows, device="cuda")
+    y = int8.AffineInt8(w.cuda(), ws.cuda(), bias.cuda()).propagate(q, scale)
+    want, bound = product64(q, scale, w.cuda(), ws.cuda(), bias.cuda(), False, None, None)
+    check_product(y, want.cpu(), bound.cpu(), torch.float32)
+    rows = (1 << 24) + 5                                                 # 4 rows to a workgroup of the row kernels
+    x = torch.randn(rows, 8, device="cuda")
+    y = int8.rms_norm(x, None, EPS)
+    h = x.double()
+    want = h / torch.sqrt(h.square().mean(1, keepdim=True) + EPS)
+    assert bool(((y.double() - want).abs() <= want.abs() * 6 * U).all())
+    q, scale = int8.quantize_rows(x)
+    top = h.abs().amax(1)
+    assert bool(((scale.double() - top / 127).abs() <= top / 127 * 6 * U).all())
+    assert bool(((q.double() * scale.double()[:, None] - h).abs() <= (top / 127)[:, None] * (0.5 + 127 * 10 * U)).all())
+
+
 def test_two_streams_use_one_layer_at_once():
     w, ws, bias, _, _ = layer_of(768, 640, 41, True)
     layer = int8.AffineInt8(w.cuda(), ws.cuda(), bias.cuda())
@@ -477,6 +517,7 @@ def test_refusals_on_the_device():
         (lambda: int8.rms_norm(x, residual=x[:5]), "shape"), (lambda: int8.rms_norm(x, residual=x.half()), "float32 expected"),
         (lambda: int8.rms_norm(x, eps=0.0), "eps"), (lambda: int8.rms_norm(x[:1].expand(6, 40)), "leading"),
         (lambda: int8.rms_norm(x, out=torch.empty(6, 41, device="cuda")), "shape"), (lambda: int8.rms_norm(x.cpu()), "on the GPU"),
+        (lambda: int8.rms_norm(x.clone().requires_grad_()), "gradient"), (lambda: layer.propagate(q, scale, torch.int8), "float32, bfloat16 or float16"),
         (lambda: int8.quantize_rows(x, ()), "offsets"), (lambda: int8.quantize_rows(x, range(9)), "offsets"),
         (lambda: int8.quantize_rows(x, out=(q[:, :39], scale)), "shape"), (lambda: int8.quantize_rows(x, out=(q, scale[:5])), "vector of 6"),
         (lambda: layer.propagate(q[:, :32], scale), "codes"), (lambda: layer.propagate(q, scale[:5]), "vector of 6"), (lambda: layer.propagate(q, scale.half()), "vector"),
@@ -491,4 +532,6 @@ def test_refusals_on_the_device():
     for call, says in bad:
         with pytest.raises(KamdError, match=says):
             call()
+    with torch.no_grad():
+        int8.rms_norm(x.clone().requires_grad_())
     torch.cuda.synchronize()
