@@ -41,10 +41,22 @@ def _fail():
     raise KamdError(_L.kamd_last_error().decode())
 
 
+# Small calls are bound by what happens here and at the launch.  So the common case -- a contiguous matrix of the right kind -- is
+# recognised by a few attribute reads; everything else, and every message, is _check's.
+
 def _matrix(t, what, dtype=None, shape=None, dev=-1):
-    """leading dimension of a matrix on the device (of this type, shape and device, where given); raises unless it is one.
-    Small calls are bound by what happens here and at the launch: a few attribute reads per tensor."""
-    if not getattr(t, "is_cuda", False):
+    """leading dimension of a matrix on the device (of this type, shape and device, where given); raises unless it is one"""
+    try:
+        if t.is_contiguous() and not t.requires_grad and (dtype is None or t.dtype is dtype):
+            if (t.shape == shape and t.get_device() == dev) if shape is not None else (t.is_cuda and t.dim() == 2):
+                return t.shape[1]
+    except (AttributeError, TypeError):
+        pass
+    return _check(t, what, dtype, shape, dev)
+
+
+def _check(t, what, dtype, shape, dev):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise KamdError("%s: a tensor on the GPU is expected" % what)
     if t.dim() != 2:
         raise KamdError("%s: a matrix is expected, got shape %s" % (what, tuple(t.shape)))
@@ -63,15 +75,22 @@ def _matrix(t, what, dtype=None, shape=None, dev=-1):
     return ld if rows > 1 or ld > cols else cols
 
 
+def _empty(rows, cols, dtype, device):
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def _empty_as(x):
     """[rows x dim] like x, without gaps between the rows"""
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return torch.empty_like(x) if x.is_contiguous() else _empty(x.shape[0], x.shape[1], x.dtype, x.device)
 
 
 def _vector(t, n, what, dev):
-    if not getattr(t, "is_cuda", False) or t.dtype is not torch.float32 or t.dim() != 1 or len(t) != n or t.get_device() != dev or not t.is_contiguous():
-        raise KamdError("%s: a contiguous float32 vector of %d on cuda:%d is expected" % (what, n, dev))
-    return t.data_ptr()
+    try:
+        if t.dtype is torch.float32 and t.get_device() == dev and t.shape == (n,) and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    raise KamdError("%s: a contiguous float32 vector of %d on cuda:%d is expected" % (what, n, dev))
 
 
 def _type(dtype, what):
@@ -97,15 +116,13 @@ def _call(dev, fn, *args):
 
 def empty_codes(rows, dim, device):
     """[rows x dim] int8 in the layout the product takes: each row begins on a multiple of 16 bytes"""
-    if dim % 16 == 0:
-        return torch.empty((rows, dim), dtype=torch.int8, device=device)
-    return torch.empty((rows, (dim + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :dim]
+    ld = (dim + 15) // 16 * 16
+    q = _empty(rows, ld, torch.int8, device)
+    return q if ld == dim else q[:, :dim]
 
 
-def _norm(x, gain, eps, residual, sum_out, out, scale):
-    """the call behind rms_norm (scale None) and rms_norm_int8; out = the output and its leading dimension, or None"""
-    L = _L or _library()
-    ld_x = _matrix(x, "x")
+def _norm(x, ld_x, gain, eps, residual, sum_out, y, ld_y, scale):
+    """the call behind rms_norm (scale None) and rms_norm_int8; returns h"""
     shape, dtype, dev = x.shape, x.dtype, x.get_device()
     rows, dim = shape
     code = _type(dtype, "x")
@@ -123,14 +140,10 @@ def _norm(x, gain, eps, residual, sum_out, out, scale):
         h = sum_out.data_ptr()
     if gain is not None:
         g = _vector(gain, dim, "gain", dev)
-    if out is None:
-        y, ld_y = _empty_as(x), dim
-    else:
-        y, ld_y = out
     if rows:
-        _call(dev, L.kamd_rms_norm_device, x.data_ptr(), ld_x, r, ld_r, code, g, eps, rows, dim, h, ld_h, y.data_ptr(), ld_y,
+        _call(dev, _L.kamd_rms_norm_device, x.data_ptr(), ld_x, r, ld_r, code, g, eps, rows, dim, h, ld_h, y.data_ptr(), ld_y,
               code if scale is None else _I8, None if scale is None else scale.data_ptr())
-    return y, sum_out
+    return sum_out
 
 
 def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
@@ -139,17 +152,20 @@ def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
     x: [rows, dim] float32 / bfloat16 / float16, rows any stride apart; residual: the same shape and type; gain: float32 [dim].
     NormalizeComponent is gain = target_rms, eps = 2^-66.  sum_out (h) and out (y) may be given; sum_out may be x or residual,
     out any of the three."""
-    if out is not None:
-        _matrix(x, "x")
-        out = out, _matrix(out, "out", x.dtype, x.shape, x.get_device())
-    y, h = _norm(x, gain, eps, residual, sum_out, out, None)
+    _L or _library()
+    ld_x = _matrix(x, "x")
+    if out is None:
+        y, ld_y = _empty_as(x), x.shape[1]
+    else:
+        y, ld_y = out, _matrix(out, "out", x.dtype, x.shape, x.get_device())
+    h = _norm(x, ld_x, gain, eps, residual, sum_out, y, ld_y, None)
     return y if h is None else (y, h)
 
 
 def _codes_out(out, rows, dim, x):
     if out is None:
         q = empty_codes(rows, dim, x.device)
-        return q, torch.empty(rows, dtype=torch.float32, device=x.device), (dim + 15) // 16 * 16
+        return q, torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device), (dim + 15) // 16 * 16
     q, scale = out
     ld_q = _matrix(q, "codes", torch.int8, (rows, dim), x.get_device())
     _vector(scale, rows, "scale", x.get_device())
@@ -158,9 +174,10 @@ def _codes_out(out, rows, dim, x):
 
 def rms_norm_int8(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
     """rms_norm with y as 8-bit rows -> (codes, scale), or (codes, scale, h) with a residual.  out = (codes, scale) may be given."""
-    _matrix(x, "x")
+    _L or _library()
+    ld_x = _matrix(x, "x")
     q, scale, ld_q = _codes_out(out, x.shape[0], x.shape[1], x)
-    _, h = _norm(x, gain, eps, residual, sum_out, (q, ld_q), scale)
+    h = _norm(x, ld_x, gain, eps, residual, sum_out, q, ld_q, scale)
     return (q, scale) if h is None else (q, scale, h)
 
 
@@ -246,7 +263,7 @@ class AffineInt8:
         s = _vector(scale, rows, "scale", dev)
         code = _type(dtype, "dtype")
         if out is None:
-            out, ld_out = torch.empty((rows, self.out_dim), dtype=dtype, device=q.device), self.out_dim
+            out, ld_out = _empty(rows, self.out_dim, dtype, self.device), self.out_dim
         else:
             ld_out = _matrix(out, "out", dtype, (rows, self.out_dim), dev)
         if rows:
