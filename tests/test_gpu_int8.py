@@ -526,7 +526,8 @@ def test_refusals_on_the_device():
         (lambda: layer.propagate(torch.zeros(5 * 48 + 40, dtype=torch.int8, device="cuda").as_strided((6, 40), (48, 1)), scale), "last row"),
         (lambda: layer.propagate(q, scale, torch.float64), "float32, bfloat16 or float16"), (lambda: layer.propagate(q, scale, out=torch.empty(6, 21, device="cuda")), "shape"),
         (lambda: layer.propagate(q, scale, torch.float16, out=torch.empty(6, 20, device="cuda")), "float16 expected"),
-        (lambda: int8.AffineInt8(w.cuda().float(), ws.cuda()), "int8 expected"), (lambda: int8.AffineInt8(w.cuda(), ws.cuda()[:19]), "vector of 20"),
+        (lambda: int8.AffineInt8(w.cuda().float(), ws.cuda()), "int8 expected"), (lambda: int8.rms_norm(x, gain=torch.ones(40, device="cuda", requires_grad=True)), "gradient"),
+        (lambda: int8.rms_norm_int8(x, out=q), "pair"), (lambda: layer.propagate(q, scale, "float"), "torch.dtype"), (lambda: int8.quantize_rows(x, (0, 2 ** 40)), "out of range"), (lambda: int8.AffineInt8(w.cuda(), ws.cuda()[:19]), "vector of 20"),
         (lambda: int8.AffineInt8(torch.zeros(2, 131072, dtype=torch.int8, device="cuda"), ws.cuda()[:2]), "131071"),
     ]
     for call, says in bad:

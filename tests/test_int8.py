@@ -85,9 +85,3 @@ def test_tensors_off_the_gpu_are_refused():
                  lambda: int8.AffineInt8(x.to(torch.int8), torch.ones(3))):
         with pytest.raises(KamdError, match="on the GPU"):
             call()
-
-
-def test_element_types_match_the_header():
-    from kaldi_amd import int8
-    assert int8._TYPES == {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16} and int8._I8 == I8
-    assert abi.KAMD_MAX_OFFSETS == 8
