@@ -205,7 +205,13 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   auto load = [&](unsigned to, i32x4 rsrc, int voff, int soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
   };
+  // Where several tiles share a CU, tiles next to each other along a row start at different places of the sum, which is exact in
+  // any order, so that not all of them ask for the same lines at once: 12000 x 1536 x 1536 36.3 -> 35.5 us, 600 x 6000 x 1536
+  // 13.9 -> 12.8.  Of no use to the other tiles, up to 3 % slower.
+  const int steps = p.kb >> 1, start = BM == 128 && NST == 2 ? (tn & 7) * 3 % steps : 0;
   auto issue = [&](int kt, int stage, int first, int last) {     // loads first .. last - 1 of this wave's for a stage
+    kt += start;
+    if (kt >= steps) kt -= steps;
     const unsigned at = lds + stage * STAGE;
 #pragma unroll
     for (int l = 0; l < LOADS; l++) {
@@ -225,7 +231,6 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   for (int i = 0; i < TI; i++)
 #pragma unroll
     for (int j = 0; j < TJ; j++) acc[i][j] = i32x4{0, 0, 0, 0};
-  const int steps = p.kb >> 1;
   const int xoff = (wm * (BM / WM) + (lane & 15)) * 128, xslot = (lane >> 4) ^ ((lane >> 1) & 7);
   const int woff = X_BYTES + wn * (BN / WN / 16) * 1024 + lane * 16;
   struct Fragments { i32x4 w[TJ], x[TI]; } half0, half1;         // 64 codes each
@@ -295,7 +300,10 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
   __syncthreads();
   unsigned char *mine = smem + wave * 16 * PITCH;
   const int nw = n0 + wn * COLS, n4 = nw + (lane >> 4) * 4;
+  // All that it reads is asked for first: a wave's loads and stores are counted in order, so that a load between the stores
+  // waits for those before it (256 x 256 tiles 3 to 6 % slower, 128 x 192 1 to 2 %).
   f32x4 w_scale[TJ], bias[TJ];
+  float x_scale[TI];
 #pragma unroll
   for (int j = 0; j < TJ; j++) {
     const int n = min(n4 + j * 16, p.np - 4);
@@ -303,12 +311,13 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
     bias[j] = *reinterpret_cast<const f32x4 *>(p.col + p.np + n);
   }
 #pragma unroll
+  for (int i = 0; i < TI; i++) x_scale[i] = p.scale[min(m0 + wm * (BM / WM) + i * 16 + (lane & 15), p.rows - 1)];
+#pragma unroll
   for (int i = 0; i < TI; i++) {
     const int mi = m0 + wm * (BM / WM) + i * 16;
-    const float scale = p.scale[min(mi + (lane & 15), p.rows - 1)];
 #pragma unroll
     for (int j = 0; j < TJ; j++) {
-      const f32x4 z = Finish(p, acc[i][j], scale, w_scale[j], bias[j], min(n4 + j * 16, p.np - 4));
+      const f32x4 z = Finish(p, acc[i][j], x_scale[i], w_scale[j], bias[j], min(n4 + j * 16, p.np - 4));
       StoreAny(mine + (lane & 15) * PITCH + ((lane >> 4) * 4 + j * 16) * sizeof(TO), __builtin_convertvector(z, OV4));
     }
     __builtin_amdgcn_wave_barrier();
@@ -372,15 +381,15 @@ void LaunchTile(AffineArgs p, hipStream_t st) {
 }
 
 // Which kernel.  A call takes about  2 us + c (s step + fixed),  c = tiles per CU, s = steps of 128 codes, with the two constants
-// of each kernel measured on MI355X; the cheapest is taken (over 80 random sizes within 3 % of the fastest of them in the mean).
+// of each kernel measured on MI355X; the cheapest is taken (over 200 random sizes within 0.5 % of the fastest of them in the mean).
 // What the kernels are for, each against its neighbour (us):
 //   16 x 16 split    1 x 4096 x 4096  3.1 (32 x 32  4.1)          20 x 320 x 7840  5.3 (7.5)
 //   32 x 32 split    24 x 6000 x 1536  3.7 (16 x 16  4.8)         64 x 4096 x 4096  6.9 (64 x 64  8.9)
 //   64 x 64, 4 st.   256 x 4096 x 4096  9.5   (64 x 128 12.1)     1000 x 768 x 768  4.0 (4.9)
 //   64 x 128, 3 st.  512 x 4096 x 4096  13.3  (64 x 64 15.7)
 //   128 x 192, 3 st. 1999 x 2328 x 1537 14.3  (64 x 128 16.6, 2 stages 16.4): one tile per CU, so that it can have all the LDS
-//   128 x 192, 2 st. 12000 x 1536 x 1536 34   (256 x 256 45.5, 3 stages 37.7): two tiles per CU cover each other's waits
-//   256 x 256, 2 st. 4096 x 4096 x 4096 55.9  (128 x 192 68.9)   16384 x 8192 x 8192  791 (921)
+//   128 x 192, 2 st. 12000 x 1536 x 1536 35.5 (256 x 256 44.6, 3 stages 40.2): two tiles per CU cover each other's waits
+//   256 x 256, 2 st. 4096 x 4096 x 4096 54.1  (128 x 192 69.4)   16384 x 8192 x 8192  791 (921)
 constexpr int kCus = 256;
 
 constexpr int kMaxRows = 1 << 22;         // per launch: the grid of the smallest tile stays within its limit
@@ -397,7 +406,7 @@ int Propagate(AffineArgs p, hipStream_t st) {
   }
   struct Kernel { int bm, bn; double step, fixed; bool alone; void (*go)(AffineArgs, hipStream_t); };     // alone: at most one tile per CU
   static const Kernel kernels[] = {{16, 16, 0.065, 0.2, false, LaunchSplit<1, 1, TO>},
-                                   {32, 32, 0.135, 0.3, false, LaunchSplit<2, 2, TO>},
+                                   {32, 32, 0.115, 0.3, false, LaunchSplit<2, 2, TO>},
                                    {64, 64, 0.19, 0.9, false, LaunchTile<64, 64, 4, 2, 4, TO>},
                                    {64, 128, 0.29, 1.2, false, LaunchTile<64, 128, 2, 4, 3, TO>},
                                    {128, 192, 0.40, 5.0, true, LaunchTile<128, 192, 2, 4, 3, TO>},
