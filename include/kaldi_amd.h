@@ -281,7 +281,7 @@ typedef struct kamd_component_i8 kamd_component_i8;
  * log-softmax; the bypass is ignored as in kamd_component. */
 kamd_component_i8 *kamd_component_i8_create(const kamd_layer_desc *layer);
 /* From weights that are coded already, d_w [out_dim x in_dim] and d_w_scale [out_dim] on the device (copied).  d_bias, d_mul
- * and d_add [out_dim] may be NULL: out = mul * relu(... + bias) + add. */
+ * and d_add [out_dim] may be NULL: out = mul * relu(... + bias) + add.  in_dim <= 131071, out_dim <= 2^26, at most 2^35 weights. */
 kamd_component_i8 *kamd_component_i8_create_quantized(const int8_t *d_w, int64_t ld_w, const float *d_w_scale, int in_dim,
                                                       int out_dim, const float *d_bias, int relu, const float *d_mul,
                                                       const float *d_add, void *stream);

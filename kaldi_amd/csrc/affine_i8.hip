@@ -30,6 +30,9 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kPadN = 256, kPadK = 128;
 constexpr int64_t kMaxIn = 131071;        // 128 * 128 * 131071 < 2^31
 constexpr int64_t kMaxLd = 1 << 23;       // a tile's rows stay within 32-bit offsets of its first
+constexpr int64_t kMaxOut = 1 << 26;      // three vectors of them stay within 32-bit indexes
+constexpr int64_t kMaxWeights = int64_t{1} << 35;
+constexpr int64_t kMaxTiles = 1 << 22;    // per launch, of 512 threads: a launch has fewer than 2^32
 
 struct AffineI8 {
   int device = 0, in_dim = 0, out_dim = 0, kp = 0, np = 0, relu = 0, mapped = 0;
@@ -416,10 +419,11 @@ int Propagate(AffineArgs p, hipStream_t st) {
   double least = 0.0;
   for (const Kernel &k : kernels) {
     const int64_t tiles = static_cast<int64_t>(CeilDiv(p.rows, k.bm)) * CeilDiv(p.n, k.bn), per_cu = (tiles + kCus - 1) / kCus;
-    if (k.alone && per_cu > 1) continue;
+    if ((k.alone && per_cu > 1) || tiles > kMaxTiles) continue;
     const double cost = static_cast<double>(per_cu) * (p.kb / 2 * k.step + k.fixed);
     if (!best || cost < least) { best = &k; least = cost; }
   }
+  if (!best) return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: %d rows of %d outputs are too many for one call", p.rows, p.n);
   best->go(p, st);
   KAMD_HIP(hipGetLastError());
   return KAMD_OK;
@@ -435,7 +439,8 @@ void Free(AffineI8 *c) {
 int CheckSizes(const char *who, int64_t in_dim, int64_t out_dim) {
   if (in_dim < 1 || out_dim < 1) return SetError(KAMD_ERR_ARG, "%s: bad sizes (%lld -> %lld)", who, static_cast<long long>(in_dim), static_cast<long long>(out_dim));
   if (in_dim > kMaxIn) return SetError(KAMD_ERR_ARG, "%s: %lld inputs: a 32-bit sum of 8-bit products holds at most %lld", who, static_cast<long long>(in_dim), static_cast<long long>(kMaxIn));
-  if (out_dim > INT32_MAX - kPadN) return SetError(KAMD_ERR_ARG, "%s: too many outputs (%lld)", who, static_cast<long long>(out_dim));
+  if (out_dim > kMaxOut || static_cast<int64_t>(RoundUp(out_dim, kPadN)) * RoundUp(in_dim, kPadK) > kMaxWeights)
+    return SetError(KAMD_ERR_ARG, "%s: too many outputs (%lld of %lld inputs)", who, static_cast<long long>(out_dim), static_cast<long long>(in_dim));
   return KAMD_OK;
 }
 

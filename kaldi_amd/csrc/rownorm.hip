@@ -236,8 +236,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void RowKernel(RowArgs a) {
 }
 
 constexpr int kMaxDim = 1 << 30;
-// At most this many workgroups per launch (rows beyond go to a launch of their own).
-constexpr int64_t kMaxGroups = 1 << 22;
+// At most this many workgroups per launch (rows beyond go to a launch of their own): a launch has fewer than 2^32 threads.
+constexpr int64_t kMaxGroups = 1 << 21;
+static_assert(kMaxGroups * 1024 < int64_t{1} << 32, "threads of a launch");
 
 template <typename T, typename TO, bool NORM, int VE, int TPR, int NV>
 static int LaunchRows(RowArgs a, hipStream_t st) {
@@ -268,6 +269,7 @@ template <typename T, typename TO, bool NORM>
 static int RunRows(const RowArgs &a, hipStream_t st) {
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
   constexpr bool I8 = sizeof(TO) == 1;
+  static_assert(KAMD_MAX_OFFSETS <= 8, "pieces");
   if (a.part_dim < VE) return LaunchRows<T, TO, NORM, 1, 64, 8>(a, st);          // at most 7 columns, in at most 8 pieces
   typedef int (*Launch)(RowArgs, hipStream_t);
   struct Shape { int tpr, ept; Launch go; };

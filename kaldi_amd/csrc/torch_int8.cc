@@ -64,10 +64,20 @@ void RefuseGradient(const at::Tensor &t, const char *what) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     Refuse(std::string(what) + ": has a gradient to keep track of, and these calls have none (torch.no_grad or detach)");
 }
+// a tensor whose values are not what its memory holds, or that has none: fake, wrapped or lazily negated ones
+void RefuseHollow(const at::Tensor &t, const char *what) {
+  if (t.key_set().has(c10::DispatchKey::Python) || !t.has_storage() || t.is_neg() || t._is_zerotensor())
+    Refuse(std::string(what) + ": a plain tensor with memory of its own is expected");
+}
+// a given output is about to be written: autograd is told, as after torch's own in-place operators
+void Written(const at::Tensor &t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Matrix Take(PyObject *o, const char *what) {
   if (!THPVariable_Check(o) || !THPVariable_Unpack(o).is_cuda()) Refuse(std::string(what) + ": a tensor on the GPU is expected");
   Matrix m;
   m.t = THPVariable_Unpack(o);
+  RefuseHollow(m.t, what);
   if (m.t.dim() != 2) Refuse(std::string(what) + ": a matrix is expected, got shape " + Shape(m.t.sizes()));
   RefuseGradient(m.t, what);
   m.rows = m.t.size(0); m.cols = m.t.size(1); m.ld = m.t.stride(0);
@@ -87,6 +97,7 @@ float *TakeVector(PyObject *o, const char *what, int64_t n, c10::Device device) 
   if (THPVariable_Check(o)) {
     const at::Tensor &t = THPVariable_Unpack(o);
     RefuseGradient(t, what);
+    RefuseHollow(t, what);
     if (t.device() == device && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.is_contiguous()) return static_cast<float *>(t.data_ptr());
   }
   Refuse(std::string(what) + ": a contiguous float32 vector of " + std::to_string(n) + " on " + device.str() + " is expected");
@@ -173,13 +184,17 @@ PyObject *RmsNorm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     else y = None(a[5]) ? Make(x.rows, x.cols, st, device) : TakeLike(a[5], "out", st, x.rows, x.cols, device);
     const Matrix &out = i8 ? codes.q : y;
     if (x.rows > 0) {
-      void *stream = Stream(device);
+      const void *from = x.data(), *added = res.data();
+      void *to_sum = sum.data(), *to = out.data(), *stream = Stream(device);
+      float *to_scale = i8 ? static_cast<float *>(codes.scale.data_ptr()) : NULL;
       int rc;
       Py_BEGIN_ALLOW_THREADS
-      rc = g_norm(x.data(), x.ld, res.data(), res.ld, type, gain, static_cast<float>(eps), x.rows, static_cast<int>(std::min<int64_t>(x.cols, INT32_MAX)),
-                  sum.data(), sum.ld, out.data(), out.ld, i8 ? KAMD_I8 : type, i8 ? static_cast<float *>(codes.scale.data_ptr()) : NULL, stream);
+      rc = g_norm(from, x.ld, added, res.ld, type, gain, static_cast<float>(eps), x.rows, static_cast<int>(std::min<int64_t>(x.cols, INT32_MAX)),
+                  to_sum, sum.ld, to, out.ld, i8 ? KAMD_I8 : type, to_scale, stream);
       Py_END_ALLOW_THREADS
       Check(rc);
+      if (!None(a[4])) Written(sum.t);
+      if (!None(a[5])) { Written(out.t); Written(codes.scale); }
     }
     PyObject *h = sum.given() ? sum.wrap() : NULL;
     if (i8) return Pack(out.wrap(), THPVariable_Wrap(codes.scale), h);
@@ -209,13 +224,17 @@ PyObject *QuantizeRows(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const c10::DeviceGuard guard(device);
     const Codes c = TakeCodes(a[2], rows, x.cols * parts, device);
     if (rows > 0) {
+      const void *from = x.data();
+      int8_t *to = static_cast<int8_t *>(c.q.data());
+      float *to_scale = static_cast<float *>(c.scale.data_ptr());
       void *stream = Stream(device);
       int rc;
       Py_BEGIN_ALLOW_THREADS
-      rc = g_quantize(x.data(), x.ld, type, x.rows, static_cast<int>(std::min<int64_t>(x.cols, INT32_MAX)), offsets, static_cast<int>(parts),
-                      static_cast<int8_t *>(c.q.data()), c.q.ld, static_cast<float *>(c.scale.data_ptr()), stream);
+      rc = g_quantize(from, x.ld, type, x.rows, static_cast<int>(std::min<int64_t>(x.cols, INT32_MAX)), offsets, static_cast<int>(parts),
+                      to, c.q.ld, to_scale, stream);
       Py_END_ALLOW_THREADS
       Check(rc);
+      if (!None(a[2])) { Written(c.q.t); Written(c.scale); }
     }
     return Pack(c.q.wrap(), THPVariable_Wrap(c.scale), NULL);
   });
@@ -236,7 +255,7 @@ PyObject *Propagate(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (q.t.scalar_type() != at::kChar) Refuse("codes: torch.int8 expected, got " + Name(q.t.scalar_type()));
     if (q.cols != in_dim || q.t.device() != device)
       Refuse("codes: [rows, " + std::to_string(in_dim) + "] on " + device.str() + " expected, got " + Shape(q.t.sizes()) + " on " + q.t.device().str());
-    if (q.rows <= 1) q.ld = (q.ld + 15) / 16 * 16;
+    if (q.rows <= 1) q.ld = (in_dim + 15) / 16 * 16;
     if (q.ld % 16 != 0 || reinterpret_cast<uintptr_t>(q.data()) % 16 != 0) Refuse("codes: rows begin on multiples of 16 bytes (int8.empty_codes has the layout)");
     if (in_dim % 16 != 0 && q.rows > 0 &&
         static_cast<int64_t>(q.t.storage().nbytes()) - q.t.storage_offset() < (q.rows - 1) * q.ld + (in_dim + 15) / 16 * 16)
@@ -245,14 +264,27 @@ PyObject *Propagate(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const c10::DeviceGuard guard(device);
     const Matrix out = None(a[7]) ? Make(q.rows, out_dim, st, device) : TakeLike(a[7], "out", st, q.rows, out_dim, device);
     if (q.rows > 0) {
-      void *stream = Stream(device);
+      const int8_t *from = static_cast<const int8_t *>(q.data());
+      void *to = out.data(), *stream = Stream(device);
       int rc;
       Py_BEGIN_ALLOW_THREADS
-      rc = g_propagate(handle, static_cast<const int8_t *>(q.data()), q.ld, scale, q.rows, out.data(), out.ld, type, stream);
+      rc = g_propagate(handle, from, q.ld, scale, q.rows, to, out.ld, type, stream);
       Py_END_ALLOW_THREADS
       Check(rc);
+      if (!None(a[7])) Written(out.t);
     }
     return out.wrap();
+  });
+}
+
+// (tensor, name): refused unless its memory holds its values
+PyObject *Plain(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return Guarded([&]() -> PyObject * {
+    if (n != 2 || !THPVariable_Check(a[0])) Refuse("plain: a tensor and its name expected");
+    const char *what = PyUnicode_AsUTF8(a[1]);
+    if (!what) throw Refused();
+    RefuseHollow(THPVariable_Unpack(a[0]), what);
+    Py_RETURN_NONE;
   });
 }
 
@@ -273,6 +305,7 @@ PyObject *Init(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 template <typename F> PyCFunction Fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)); }
 PyMethodDef g_methods[] = {{"init", Fast(Init), METH_FASTCALL, NULL},
+                           {"plain", Fast(Plain), METH_FASTCALL, NULL},
                            {"rms_norm", Fast(RmsNorm), METH_FASTCALL, NULL},
                            {"quantize_rows", Fast(QuantizeRows), METH_FASTCALL, NULL},
                            {"propagate", Fast(Propagate), METH_FASTCALL, NULL},

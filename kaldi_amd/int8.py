@@ -58,7 +58,8 @@ def empty_codes(rows, dim, device):
 
 
 def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
-    """y = h / sqrt(mean(h^2) + eps) * gain per row, h = x + residual -> y, or (y, h) with a residual (kamd_rms_norm_device).
+    """y = h / sqrt(mean(h^2) + eps) * gain per row, h = x + residual -> y, or (y, h) with a residual or sum_out
+    (kamd_rms_norm_device).
 
     x: [rows, dim] float32 / bfloat16 / float16, rows any stride apart; residual: the same shape and type; gain: float32 [dim].
     NormalizeComponent is gain = target_rms, eps = 2^-66.  sum_out (h) and out (y) may be given; sum_out may be x or residual,
@@ -67,7 +68,8 @@ def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
 
 
 def rms_norm_int8(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
-    """rms_norm with y as 8-bit rows -> (codes, scale), or (codes, scale, h) with a residual.  out = (codes, scale) may be given."""
+    """rms_norm with y as 8-bit rows -> (codes, scale), or (codes, scale, h) with a residual or sum_out.  out = (codes, scale)
+    may be given."""
     return (_X or _extension()).rms_norm(x, gain, eps, residual, sum_out, out, True)
 
 
@@ -80,6 +82,7 @@ def quantize_rows(x, offsets=(0,), out=None):
 def _vector(t, n, what, device):
     if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise KamdError("%s: a contiguous float32 vector of %d on %s is expected" % (what, n, device))
+    _extension().plain(t, what)
     return t.data_ptr()
 
 
@@ -95,6 +98,7 @@ class AffineInt8:
             raise KamdError("weight: a tensor on the GPU is expected")
         if weight.dtype != torch.int8 or weight.dim() != 2:
             raise KamdError("weight: a matrix of torch.int8 expected, got %s %s" % (weight.dtype, tuple(weight.shape)))
+        _extension().plain(weight, "weight")
         weight = weight.contiguous()
         n, k = weight.shape
         vectors = [None if v is None else _vector(v, n, what, weight.device) for v, what in
@@ -128,6 +132,9 @@ class AffineInt8:
         if getattr(self, "_h", None) and _L is not None:
             _L.kamd_component_i8_destroy(self._h)
             self._h = None
+
+    def __reduce__(self):
+        raise KamdError("AffineInt8: a handle to device memory; neither copied nor pickled")
 
     def quantize_input(self, x, out=None):
         """the codes and scales of the layer's spliced input"""

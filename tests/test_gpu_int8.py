@@ -536,3 +536,45 @@ def test_refusals_on_the_device():
     with torch.no_grad():
         int8.rms_norm(x.clone().requires_grad_())
     torch.cuda.synchronize()
+
+
+def test_given_outputs_count_as_written():
+    """what autograd saved of a tensor that a call writes into is stale, and has to be known as such"""
+    x = torch.randn(3, 64, device="cuda")
+    w = torch.randn(64, 64, device="cuda", requires_grad=True)
+    loss = (x @ w).sum()                      # saves x
+    h, codes, y = x.clone(), (int8.empty_codes(3, 64, "cuda"), torch.empty(3, device="cuda")), torch.empty(3, 64, device="cuda")
+    before = [t._version for t in (h, *codes, y)]
+    int8.rms_norm(x, sum_out=h, out=y)
+    int8.quantize_rows(x, out=codes)
+    assert [t._version - b for t, b in zip((h, *codes, y), before)] == [1, 1, 1, 1]
+    assert x._version == 0
+    int8.rms_norm(x, residual=x, sum_out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        z = torch.randn(3, 64, device="cuda")
+    int8.rms_norm(z, out=z)                   # has no count to keep
+
+
+def test_one_row_of_a_matrix_whose_rows_lie_far_apart():
+    big = torch.zeros(2, 1 << 24, dtype=torch.int8, device="cuda")
+    row = big[1:, :48]
+    row.copy_(torch.arange(-24, 24, dtype=torch.int8, device="cuda")[None])
+    layer = int8.AffineInt8(torch.eye(48, dtype=torch.int8, device="cuda"), torch.ones(48, device="cuda"))
+    y = layer.propagate(row, torch.full((1,), 0.5, device="cuda"))
+    assert torch.equal(y, row.float() * 0.5)
+
+
+@pytest.mark.parametrize("k", [1, 64, 128, 129, 384, 1000])
+def test_sums_that_start_in_the_middle(k):
+    """128 x 192 tiles side by side begin at different places of the sum: every column of tiles, sums from one stage upwards"""
+    rows, n = 2030, 192 * 31 + 187            # two tiles per CU
+    g = torch.Generator().manual_seed(k)
+    q = int8.empty_codes(rows, k, "cuda")
+    q.copy_(torch.randint(-127, 128, (rows, k), generator=g, dtype=torch.int8))
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+    layer = int8.AffineInt8(w.cuda(), torch.ones(n, device="cuda"))
+    y = layer.propagate(q, torch.full((rows,), 2.0 ** -20, device="cuda"))
+    # |sum| <= 1000 * 127^2 < 2^24: exact in 32-bit floats, and so is the power of two
+    assert torch.equal(y.cpu().double(), (q.cpu().double() @ w.double().T) * 2.0 ** -20)

@@ -85,3 +85,34 @@ def test_tensors_off_the_gpu_are_refused():
                  lambda: int8.AffineInt8(x.to(torch.int8), torch.ones(3))):
         with pytest.raises(KamdError, match="on the GPU"):
             call()
+
+
+def test_widths_a_launch_cannot_take_are_refused():
+    L = lib()
+    for in_dim, out_dim in ((8, 2 ** 26 + 1), (131071, 2 ** 18 + 1), (100000, 2 ** 26)):
+        assert not L.kamd_component_i8_create_quantized(P, in_dim, P, in_dim, out_dim, None, 0, None, None, None)
+        assert "too many outputs" in L.kamd_last_error().decode()
+
+
+def test_tensors_without_memory_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    with FakeTensorMode():
+        x, w, v = torch.empty(3, 8, device="cuda"), torch.empty(4, 8, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
+    for call in (lambda: int8.rms_norm(x), lambda: int8.rms_norm_int8(x), lambda: int8.quantize_rows(x), lambda: int8.AffineInt8(w, v)):
+        with pytest.raises(KamdError, match="plain tensor"):
+            call()
+
+
+def test_a_handle_is_not_copied():
+    import copy
+    import pickle
+
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    layer = int8.AffineInt8.__new__(int8.AffineInt8)
+    for call in (lambda: copy.copy(layer), lambda: copy.deepcopy(layer), lambda: pickle.dumps(layer)):
+        with pytest.raises(KamdError, match="neither copied nor pickled"):
+            call()
