@@ -102,8 +102,8 @@ __device__ inline void TileOf(int b, int tiles_m, int tiles_n, int *tm, int *tn)
 
 // Few rows, or few tiles: what counts is how many loads are under way at once.  A workgroup computes 16 TI rows x 16 TJ channels;
 // each of its 8 waves takes every 8th block of 64 codes of all of them, operands straight into registers, with no barrier until
-// the sums are joined in LDS.
-template <int TI, int TJ, typename TO>
+// the sums are joined in LDS.  ONCE: the weights are read once by the call and not kept for the next.
+template <int TI, int TJ, bool ONCE, typename TO>
 __global__ __launch_bounds__(512) void SplitKernel(AffineArgs p) {
   constexpr int NW = 8, U = TI * TJ <= 2 ? 4 : 2;                // U blocks are loaded before the first is multiplied
   __shared__ i32x4 part[NW][TI * TJ][64];
@@ -128,7 +128,10 @@ __global__ __launch_bounds__(512) void SplitKernel(AffineArgs p) {
       if (k0 + u * NW < p.kb) {
         const int k = k0 + u * NW, at = min(k * 64 + chunk, p.last_chunk);
 #pragma unroll
-        for (int j = 0; j < TJ; j++) a[u][j] = *reinterpret_cast<const i32x4 *>(w + (static_cast<size_t>(k) * 16 + j) * 1024);
+        for (int j = 0; j < TJ; j++) {
+          const i32x4 *block = reinterpret_cast<const i32x4 *>(w + (static_cast<size_t>(k) * 16 + j) * 1024);
+          a[u][j] = ONCE ? __builtin_nontemporal_load(block) : *block;
+        }
 #pragma unroll
         for (int i = 0; i < TI; i++) b[u][i] = *reinterpret_cast<const i32x4 *>(x[i] + at);
       }
@@ -362,10 +365,19 @@ __global__ __launch_bounds__(256) void ColumnsKernel(const float *w_scale, const
   to[3 * np + i] = in && add ? add[i] : 0.0f;
 }
 
+// Weights that the L2s (8 x 4 MB) cannot hold until the next call pass them by where one tile of at most 16 rows reads them once
+// (us from HBM, in brackets from the last-level cache):  1 x 8192 x 8192  13.7 -> 12.1 (11.1 -> 11.3),  16 x 8192 x 8192  14.6 -> 13.3
+// (11.9 -> 12.8).  Not from 24 rows on, 16.3 -> 15.1 (12.3 -> 14.6), nor smaller ones:  1 x 4096 x 4096  5.0 -> 4.8 (L2s 3.1 -> 4.5).
+constexpr int64_t kL2Bytes = 32 << 20;
+
 template <int TI, int TJ, typename TO>
 void LaunchSplit(AffineArgs p, hipStream_t st) {
   p.tiles_m = CeilDiv(p.rows, TI * 16); p.tiles_n = CeilDiv(p.n, TJ * 16);
-  hipLaunchKernelGGL((SplitKernel<TI, TJ, TO>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
+  const dim3 grid(p.tiles_m * p.tiles_n), block(512);
+  if (p.rows <= 16 && static_cast<int64_t>(p.np) * p.kb * 64 > kL2Bytes)
+    hipLaunchKernelGGL((SplitKernel<TI, TJ, true, TO>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((SplitKernel<TI, TJ, false, TO>), grid, block, 0, st, p);
 }
 
 // An output that the last-level cache (256 MB) could not keep for the next layer anyway goes past the caches, whose lines the

@@ -578,3 +578,19 @@ def test_sums_that_start_in_the_middle(k):
     y = layer.propagate(q, torch.full((rows,), 2.0 ** -20, device="cuda"))
     # |sum| <= 1000 * 127^2 < 2^24: exact in 32-bit floats, and so is the power of two
     assert torch.equal(y.cpu().double(), (q.cpu().double() @ w.double().T) * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, k, n", [(1, 4200, 8193), (16, 8000, 4500), (17, 4200, 8193), (3, 1000, 40000)])
+def test_few_rows_of_large_weights(rows, k, n, dtype):
+    """weights beyond the L2s, which up to 16 rows read past them"""
+    g = torch.Generator().manual_seed(rows)
+    q = int8.empty_codes(rows, k, "cuda")
+    q.copy_(torch.randint(-15, 16, (rows, k), generator=g, dtype=torch.int8))
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+    layer = int8.AffineInt8(w.cuda(), torch.ones(n, device="cuda"))
+    scale = torch.full((rows,), 2.0 ** -20, device="cuda")
+    # |sum| <= 8000 * 15 * 127 < 2^24: exact in 32-bit floats, so that the output's type rounds an exact value once
+    want = ((q.cpu().float() @ w.float().T).double() * 2.0 ** -20).to(dtype)
+    for _ in range(3):
+        assert torch.equal(layer.propagate(q, scale, dtype).cpu(), want)
