@@ -64,9 +64,10 @@ void RefuseGradient(const at::Tensor &t, const char *what) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     Refuse(std::string(what) + ": has a gradient to keep track of, and these calls have none (torch.no_grad or detach)");
 }
-// a tensor whose values are not what its memory holds, or that has none: fake, wrapped or lazily negated ones
+// a tensor whose values are not what its memory holds, or that has none: fake, wrapped (by a subclass or by functionalization,
+// whose null pointer would read as an argument that is not given) or lazily negated ones
 void RefuseHollow(const at::Tensor &t, const char *what) {
-  if (t.key_set().has(c10::DispatchKey::Python) || !t.has_storage() || t.is_neg() || t._is_zerotensor())
+  if (t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize})) || !t.has_storage() || t.is_neg() || t._is_zerotensor())
     Refuse(std::string(what) + ": a plain tensor with memory of its own is expected");
 }
 // a given output is about to be written: autograd is told, as after torch's own in-place operators

@@ -116,3 +116,24 @@ def test_a_handle_is_not_copied():
     for call in (lambda: copy.copy(layer), lambda: copy.deepcopy(layer), lambda: pickle.dumps(layer)):
         with pytest.raises(KamdError, match="neither copied nor pickled"):
             call()
+
+
+def refused(t, says):
+    """what the calls look at in each of their tensors before anything else, on a tensor of the CPU"""
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    with pytest.raises(KamdError, match=says):
+        int8._extension().plain(t, "t")
+
+
+def test_wrappers_of_functionalization_are_refused():
+    """their data_ptr() is null, which the C entries read as an argument that is not given"""
+    seen = []
+
+    def look(t):
+        seen.append(t.data_ptr())
+        refused(t, "plain tensor")
+        return t + 1
+
+    assert torch.func.functionalize(look)(torch.ones(4)).tolist() == [2.0] * 4
+    assert seen == [0]
