@@ -69,6 +69,11 @@ void RefuseGradient(const at::Tensor &t, const char *what) {
 void RefuseHollow(const at::Tensor &t, const char *what) {
   if (t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize})) || !t.has_storage() || t.is_neg() || t._is_zerotensor())
     Refuse(std::string(what) + ": a plain tensor with memory of its own is expected");
+  // the memory can be shorter than what the shape spans: untyped_storage().resize_() leaves the tensors on it as they were
+  int64_t span = t.numel() == 0 ? 0 : 1;
+  for (int64_t d = 0; span > 0 && d < t.dim(); d++) span += (t.size(d) - 1) * t.stride(d);
+  if (span > 0 && static_cast<int64_t>(t.storage().nbytes()) < (t.storage_offset() + span) * static_cast<int64_t>(t.itemsize()))
+    Refuse(std::string(what) + ": its storage is shorter than the tensor");
 }
 // a given output is about to be written: autograd is told, as after torch's own in-place operators
 void Written(const at::Tensor &t) {

@@ -137,3 +137,19 @@ def test_wrappers_of_functionalization_are_refused():
 
     assert torch.func.functionalize(look)(torch.ones(4)).tolist() == [2.0] * 4
     assert seen == [0]
+
+
+@pytest.mark.parametrize("left", [0, 16, 4 * 33 - 1])
+def test_tensors_on_too_short_a_storage_are_refused(left):
+    """a storage that was resized under its tensors: without memory their pointer is null, with some of it the rest would be read"""
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    whole = torch.zeros(6, 8)
+    t = whole[1:5, 1:5]                       # spans elements 9 .. 36
+    int8._extension().plain(t, "t")
+    whole.untyped_storage().resize_(4 * 37)
+    int8._extension().plain(t, "t")
+    whole.untyped_storage().resize_(left)
+    with pytest.raises(KamdError, match="shorter than the tensor"):          # (here: a failure prints no values of t)
+        int8._extension().plain(t, "t")
+    int8._extension().plain(torch.empty(0, 8), "t")
