@@ -153,3 +153,15 @@ def test_tensors_on_too_short_a_storage_are_refused(left):
     with pytest.raises(KamdError, match="shorter than the tensor"):          # (here: a failure prints no values of t)
         int8._extension().plain(t, "t")
     int8._extension().plain(torch.empty(0, 8), "t")
+
+
+def test_vectors_that_ask_for_a_gradient_are_refused():
+    """a layer's bias, maps and scales are copied into the handle: what is learned of them would be lost"""
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    v = torch.ones(4, requires_grad=True)
+    with pytest.raises(KamdError, match="bias: has a gradient"):
+        int8._vector(v, 4, "bias", torch.device("cpu"))
+    with torch.no_grad():
+        assert int8._vector(v, 4, "bias", torch.device("cpu")) == v.data_ptr()
+    assert int8._vector(v.detach(), 4, "bias", torch.device("cpu")) == v.data_ptr()
