@@ -10,6 +10,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <algorithm>
@@ -63,6 +64,8 @@ struct Matrix {
 void RefuseGradient(const at::Tensor &t, const char *what) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     Refuse(std::string(what) + ": has a gradient to keep track of, and these calls have none (torch.no_grad or detach)");
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    Refuse(std::string(what) + ": has a tangent (forward-mode gradient) to carry on, and these calls have none (detach)");
 }
 // a tensor whose values are not what its memory holds, or that has none: fake, wrapped (by a subclass or by functionalization,
 // whose null pointer would read as an argument that is not given) or lazily negated ones

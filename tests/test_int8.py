@@ -165,3 +165,15 @@ def test_vectors_that_ask_for_a_gradient_are_refused():
     with torch.no_grad():
         assert int8._vector(v, 4, "bias", torch.device("cpu")) == v.data_ptr()
     assert int8._vector(v.detach(), 4, "bias", torch.device("cpu")) == v.data_ptr()
+
+
+def test_tensors_with_a_tangent_are_refused():
+    import torch.autograd.forward_ad as fw
+    from kaldi_amd import int8
+    with fw.dual_level():
+        t = fw.make_dual(torch.ones(4), torch.ones(4))
+        refused(t, "tangent")
+        with torch.no_grad():                     # (which switches the other direction off only)
+            refused(t, "tangent")
+        int8._extension().plain(t.detach(), "t")
+        int8._extension().plain(fw.unpack_dual(t).primal, "t")
