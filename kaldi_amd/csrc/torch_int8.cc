@@ -7,11 +7,13 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty_strided.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <algorithm>
 #include <string>
@@ -61,6 +63,13 @@ struct Matrix {
   PyObject *wrap() const { return THPVariable_Wrap(t); }
 };
 
+// While torch records what is computed, these calls, no operators of torch's, would be left out and their results kept as constants.
+void RefuseTracing() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL))
+    Refuse("kaldi_amd.int8: these calls cannot be traced (torch.jit.trace, make_fx, FakeTensorMode)");
+}
 void RefuseGradient(const at::Tensor &t, const char *what) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     Refuse(std::string(what) + ": has a gradient to keep track of, and these calls have none (torch.no_grad or detach)");
@@ -175,6 +184,7 @@ Codes TakeCodes(PyObject *out, int64_t rows, int64_t cols, c10::Device device) {
 PyObject *RmsNorm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject * {
     if (n != 7) Refuse("rms_norm: 7 arguments expected");
+    RefuseTracing();
     const Matrix x = Take(a[0], "x");
     const c10::Device device = x.t.device();
     const at::ScalarType st = x.t.scalar_type();
@@ -215,6 +225,7 @@ PyObject *RmsNorm(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyObject *QuantizeRows(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject * {
     if (n != 3) Refuse("quantize_rows: 3 arguments expected");
+    RefuseTracing();
     const Matrix x = Take(a[0], "x");
     const c10::Device device = x.t.device();
     const int type = Type(x.t.scalar_type(), "x");
@@ -253,6 +264,7 @@ PyObject *QuantizeRows(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyObject *Propagate(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject * {
     if (n != 8) Refuse("propagate: 8 arguments expected");
+    RefuseTracing();
     const kamd_component_i8 *handle = static_cast<const kamd_component_i8 *>(PyLong_AsVoidPtr(a[0]));
     const int64_t in_dim = PyLong_AsLongLong(a[1]), out_dim = PyLong_AsLongLong(a[2]);
     const c10::Device device(c10::DeviceType::CUDA, static_cast<c10::DeviceIndex>(PyLong_AsLong(a[3])));
@@ -290,6 +302,7 @@ PyObject *Propagate(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyObject *Plain(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return Guarded([&]() -> PyObject * {
     if (n != 2 || !THPVariable_Check(a[0])) Refuse("plain: a tensor and its name expected");
+    RefuseTracing();
     const char *what = PyUnicode_AsUTF8(a[1]);
     if (!what) throw Refused();
     RefuseHollow(THPVariable_Unpack(a[0]), what);

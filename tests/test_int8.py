@@ -177,3 +177,29 @@ def test_tensors_with_a_tangent_are_refused():
             refused(t, "tangent")
         int8._extension().plain(t.detach(), "t")
         int8._extension().plain(fw.unpack_dual(t).primal, "t")
+
+
+def test_calls_are_refused_while_torch_records():
+    """a trace would hold their results as constants"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    calls = []
+
+    def look(t):
+        for call in (lambda: int8.rms_norm(t), lambda: int8.rms_norm_int8(t), lambda: int8.quantize_rows(t), lambda: int8._vector(t, 4, "t", t.device),
+                     lambda: int8._extension().propagate(0, 4, 4, 0, t, t, torch.float32, None)):
+            with pytest.raises(KamdError, match="cannot be traced"):
+                call()
+            calls.append(t)
+        return t + 1
+
+    x = torch.ones(4)
+    torch.jit.trace(look, x, check_trace=False)
+    make_fx(look)(x)
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        look(x)
+    assert len(calls) == 15
+    int8._extension().plain(x, "x")
