@@ -99,8 +99,10 @@ class AffineInt8:
         if weight.dtype != torch.int8 or weight.dim() != 2:
             raise KamdError("weight: a matrix of torch.int8 expected, got %s %s" % (weight.dtype, tuple(weight.shape)))
         _extension().plain(weight, "weight")
-        weight = weight.contiguous()
         n, k = weight.shape
+        if max(n, k) > 2 ** 31 - 1:               # (the C entry takes ints, to which ctypes cuts what it is given)
+            raise KamdError("weight: %d x %d is too large" % (n, k))
+        weight = weight.contiguous()
         vectors = [None if v is None else _vector(v, n, what, weight.device) for v, what in
                    ((weight_scale, "weight_scale"), (bias, "bias"), (mul, "mul"), (add, "add"))]
         self.device, self.offsets = weight.device, (0,)

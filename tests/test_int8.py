@@ -203,3 +203,16 @@ def test_calls_are_refused_while_torch_records():
         look(x)
     assert len(calls) == 15
     int8._extension().plain(x, "x")
+
+
+@pytest.mark.parametrize("shape", [(1, 2 ** 32 + 8), (2 ** 32 + 3, 1), (2 ** 31, 1)])
+def test_weights_of_more_than_an_int_are_refused(shape):
+    """(1, 2^32 + 8) was a layer of 8 inputs"""
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+
+    class OnGpu(torch.Tensor):                    # is asked where it lives before its size
+        is_cuda = True
+    w = torch.zeros(1, dtype=torch.int8).expand(shape).as_subclass(OnGpu)
+    with pytest.raises(KamdError, match="weight: %d x %d is too large" % shape):
+        int8.AffineInt8(w, torch.ones(1).expand(shape[0]))
