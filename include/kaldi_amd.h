@@ -265,7 +265,8 @@ enum { KAMD_F32 = 0, KAMD_BF16 = 1, KAMD_F16 = 2, KAMD_I8 = 3 };
  * floor is eps = 2^-66.  h is the 32-bit sum, also where d_sum rounds it to 16 bits, and codes are made of the 32-bit h * gain.  out_type is `type`, or KAMD_I8: then out
  * holds codes in [-127, 127] and d_out_scale[row] their scale: out ~ code * scale, off by at most scale / 2; a row of zeros has
  * scale 0, one that holds an infinity or a NaN has scale NaN (and codes 0).  d_sum may be d_x or d_residual, and d_out (of the
- * input's type) any of the three, at the same leading dimension; other overlaps are not allowed. */
+ * input's type) any of the three, at the same leading dimension; any other overlap of an output with another argument is refused,
+ * here and in the calls below. */
 int kamd_rms_norm_device(const void *d_x, int64_t ld_x, const void *d_residual, int64_t ld_residual, int type,
                          const float *d_gain, float eps, int64_t rows, int dim, void *d_sum, int64_t ld_sum,
                          void *d_out, int64_t ld_out, int out_type, float *d_out_scale, void *stream);

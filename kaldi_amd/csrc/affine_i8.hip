@@ -550,6 +550,9 @@ int kamd_component_i8_propagate(const kamd_component_i8 *h, const int8_t *d_q, i
     return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: rows of codes begin on multiples of 16 bytes, at most %lld apart", static_cast<long long>(kamd::kMaxLd));
   if (rows == 0) return KAMD_OK;
   if (!d_q || !d_scale || !d_out) return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: null argument");
+  const kamd::MemoryRows out = kamd::RowsOf(d_out, ld_out, c->out_dim, out_type == KAMD_F32 ? 4 : 2, rows);
+  if (RowsMeet(out, kamd::RowsOf(d_q, ld_q, c->in_dim, 1, rows)) || RowsMeet(out, kamd::RowsOf(d_scale, rows, rows, 4, 1)))
+    return SetError(KAMD_ERR_ARG, "kamd_component_i8_propagate: the output overlaps another argument");
   int device = -1;
   KAMD_HIP(hipGetDevice(&device));
   if (device != c->device) return SetError(KAMD_ERR_STATE, "kamd_component_i8_propagate: the handle belongs to device %d, the current one is %d", c->device, device);

@@ -43,6 +43,33 @@ struct AbortHook {
 }  // namespace
 
 namespace kamd {
+bool RowsMeet(const MemoryRows &x, const MemoryRows &y) {
+  if (!x.p || !y.p || x.width <= 0 || y.width <= 0 || x.rows <= 0 || y.rows <= 0) return false;
+  const bool in_order = reinterpret_cast<uintptr_t>(x.p) <= reinterpret_cast<uintptr_t>(y.p);
+  const MemoryRows &a = in_order ? x : y, &b = in_order ? y : x;                // a begins first, b begins `d` bytes behind it
+  const uintptr_t d = reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p);
+  auto end = [](const MemoryRows &m) { return static_cast<uintptr_t>(m.rows - 1) * m.ld + m.width; };
+  if (d >= end(a)) return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.ld == b.ld || a.rows == 1 || b.rows == 1) {
+    // columns of one matrix side by side: b's first byte lies in a's row d / ld (there is such a row, d being inside a)
+    const uintptr_t ld = a.rows == 1 ? b.ld : a.ld, at = d % ld;
+    if (a.rows == 1) return true;                                               // d < width of the one row
+    return at < static_cast<uintptr_t>(a.width) || at + b.width > ld;           // in that row, or reaching into the next
+  }
+  // row by row of the one that has fewer: the last row of the other that begins before this one's end
+  const bool few_a = a.rows <= b.rows;
+  const MemoryRows &f = few_a ? a : b, &o = few_a ? b : a;
+  const intptr_t at0 = few_a ? -static_cast<intptr_t>(d) : static_cast<intptr_t>(d);     // f's first byte, from o's
+  for (int64_t i = 0; i < f.rows; i++) {
+    const intptr_t first = at0 + i * f.ld, last = first + f.width - 1;
+    if (last < 0) continue;
+    const intptr_t row = std::min<intptr_t>(last / o.ld, o.rows - 1);
+    if (row * o.ld + o.width > first) return true;
+  }
+  return false;
+}
+
 namespace {
 // A small pool of page-locked bounce buffers: a copy takes one, the pool's lock is held only while a buffer changes hands
 // (never across a copy or a stream wait: a thread waiting for a long-running stream must not hold up the host-tail threads'

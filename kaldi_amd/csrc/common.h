@@ -87,6 +87,16 @@ inline T *DevAlloc(size_t n) {
 inline int CeilDiv(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 inline int RoundUp(int a, int b) { return ((a + b - 1) / b) * b; }
 
+// A matrix in memory, in bytes (width = 0: none).  A call whose kernel runs over all its rows at once cannot have one of its
+// outputs lie over another of its arguments, unless the same thread reads and writes the same element of both.
+struct MemoryRows {
+  const void *p;
+  int64_t ld, width, rows;
+};
+inline MemoryRows RowsOf(const void *p, int64_t ld, int64_t cols, int size, int64_t rows) { return {p, (rows > 1 ? ld : cols) * size, p ? cols * size : 0, rows}; }
+bool RowsMeet(const MemoryRows &a, const MemoryRows &b);         // some byte belongs to both; common.cc
+inline bool SameRows(const MemoryRows &a, const MemoryRows &b) { return a.p == b.p && a.width == b.width && a.rows == b.rows && a.ld == b.ld; }
+
 // ---- device helpers -------------------------------------------------------
 // order-preserving float <-> uint map (for atomicMin on costs, radix select)
 __host__ __device__ inline uint32_t FloatToOrdered(float f) {

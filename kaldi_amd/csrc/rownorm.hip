@@ -306,6 +306,14 @@ int kamd_rms_norm_device(const void *d_x, int64_t ld_x, const void *d_residual, 
   if (rows == 0) return KAMD_OK;
   if (!d_x || !d_out) return SetError(KAMD_ERR_ARG, "kamd_rms_norm_device: null argument");
   if (out_type == KAMD_I8 && !d_out_scale) return SetError(KAMD_ERR_ARG, "kamd_rms_norm_device: 8-bit output needs d_out_scale");
+  const int size = type == KAMD_F32 ? 4 : 2, out_size = out_type == KAMD_I8 ? 1 : size;
+  const kamd::MemoryRows x = kamd::RowsOf(d_x, ld_x, dim, size, rows), residual = kamd::RowsOf(d_residual, ld_residual, dim, size, rows),
+                         sum = kamd::RowsOf(d_sum, ld_sum, dim, size, rows), out = kamd::RowsOf(d_out, ld_out, dim, out_size, rows),
+                         scale = kamd::RowsOf(out_type == KAMD_I8 ? d_out_scale : NULL, rows, rows, 4, 1), gain = kamd::RowsOf(d_gain, dim, dim, 4, 1);
+  auto apart = [](const kamd::MemoryRows &a, const kamd::MemoryRows &b) { return kamd::SameRows(a, b) || !kamd::RowsMeet(a, b); };
+  bool fine = apart(sum, x) && apart(sum, residual) && apart(out, x) && apart(out, residual) && apart(out, sum) && !RowsMeet(sum, gain) && !RowsMeet(out, gain);
+  for (const kamd::MemoryRows &m : {x, residual, sum, out, gain}) fine = fine && !RowsMeet(scale, m);
+  if (!fine) return SetError(KAMD_ERR_ARG, "kamd_rms_norm_device: an output overlaps another argument (it may lie exactly on a matrix of its own type)");
   if (!kamd::RequireDevice()) return KAMD_ERR_HIP;
   kamd::RowArgs a = {};
   a.x = d_x; a.residual = d_residual; a.sum = d_sum; a.out = d_out; a.out_scale = out_type == KAMD_I8 ? d_out_scale : NULL; a.gain = d_gain;
@@ -331,10 +339,14 @@ int kamd_quantize_rows_device(const void *d_x, int64_t ld_x, int type, int64_t i
     return SetError(KAMD_ERR_ARG, "kamd_quantize_rows_device: leading dimension smaller than the matrix");
   if (in_rows <= hi - lo) return KAMD_OK;                        // no row has all its context
   if (!d_x || !d_q || !d_scale) return SetError(KAMD_ERR_ARG, "kamd_quantize_rows_device: null argument");
+  const int64_t n = static_cast<int64_t>(dim) * n_offsets, rows = in_rows - (hi - lo);
+  const kamd::MemoryRows x = kamd::RowsOf(d_x, ld_x, dim, type == KAMD_F32 ? 4 : 2, in_rows), q = kamd::RowsOf(d_q, ld_q, n, 1, rows),
+                         scale = kamd::RowsOf(d_scale, rows, rows, 4, 1);
+  if (RowsMeet(q, x) || RowsMeet(scale, x) || RowsMeet(scale, q)) return SetError(KAMD_ERR_ARG, "kamd_quantize_rows_device: an output overlaps another argument");
   if (!kamd::RequireDevice()) return KAMD_ERR_HIP;
   kamd::RowArgs a = {};
   a.x = d_x; a.ld_x = ld_x; a.out = d_q; a.ld_out = ld_q; a.out_scale = d_scale;
-  a.rows = in_rows - (hi - lo); a.part_dim = dim; a.n_parts = n_offsets;
+  a.rows = rows; a.part_dim = dim; a.n_parts = n_offsets;
   for (int i = 0; i < n_offsets; i++) a.part_at[i] = (offsets[i] - lo) * ld_x;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (type == KAMD_F32) return kamd::RunRows<float, int8_t, false>(a, st);

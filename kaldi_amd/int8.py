@@ -63,7 +63,7 @@ def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
 
     x: [rows, dim] float32 / bfloat16 / float16, rows any stride apart; residual: the same shape and type; gain: float32 [dim].
     NormalizeComponent is gain = target_rms, eps = 2^-66.  sum_out (h) and out (y) may be given; sum_out may be x or residual,
-    out any of the three."""
+    out any of the three.  Any other overlap of an output with another argument is refused, here and in the calls below."""
     return (_X or _extension()).rms_norm(x, gain, eps, residual, sum_out, out, False)
 
 

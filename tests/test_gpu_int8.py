@@ -594,3 +594,37 @@ def test_few_rows_of_large_weights(rows, k, n, dtype):
     want = ((q.cpu().float() @ w.float().T).double() * 2.0 ** -20).to(dtype)
     for _ in range(3):
         assert torch.equal(layer.propagate(q, scale, dtype).cpu(), want)
+
+
+def test_outputs_over_other_arguments_are_refused():
+    """views of one buffer: outputs beside the inputs are written there, over them they are refused"""
+    w, ws, _, _, _ = layer_of(48, 24, 71, True)
+    layer = int8.AffineInt8(w.cuda(), ws.cuda())
+    b = rand(9, 100, seed=72).cuda()
+    x, gain = b[:, :40], torch.ones(40, device="cuda")
+    want = int8.rms_norm(x.clone(), gain, EPS)
+    y = int8.rms_norm(x, gain, EPS, out=b[:, 40:80])                     # the columns beside x
+    assert torch.equal(y, want) and torch.equal(b[:, 40:80], want)
+    mem = torch.zeros(9 * 48, dtype=torch.int8, device="cuda")
+    q, scale = int8.quantize_rows(rand(9, 48, seed=73).cuda(), out=(mem.view(9, 48), torch.empty(9, device="cuda")))
+    bad = [
+        lambda: int8.rms_norm(x, gain, EPS, out=b[:, 39:79]), lambda: int8.rms_norm(x[1:], gain, EPS, out=x[:-1]), lambda: int8.rms_norm(x, gain, EPS, out=b.as_strided((9, 40), (99, 1), 62)),
+        lambda: int8.rms_norm(x, gain, EPS, residual=b[:, 1:41], sum_out=x), lambda: int8.rms_norm(x, b[0, 50:90], EPS, sum_out=b[:, 45:85]),
+        lambda: int8.rms_norm_int8(x, gain, EPS, out=(b.view(torch.int8)[:, 100:140], torch.empty(9, device="cuda"))),
+        lambda: int8.quantize_rows(x, out=(b.view(torch.int8)[:, 159:199], torch.empty(9, device="cuda"))),
+        lambda: int8.quantize_rows(x, out=(torch.empty(9, 40, dtype=torch.int8, device="cuda"), b[0, 20:29])),
+        lambda: layer.propagate(q[:1], scale[:1], out=mem.view(torch.float32)[:24].view(1, 24)),
+        lambda: layer.propagate(q[:1], scale[:1], torch.float16, out=mem[46:94].view(torch.float16).view(1, 24)),
+        lambda: layer.propagate(q[:1], b[0, 20:21], out=b[0, :24].view(1, 24)),
+    ]
+    before = b.clone(), mem.clone()
+    for call in bad:
+        with pytest.raises(KamdError, match="overlaps"):
+            call()
+    assert torch.equal(b, before[0]) and torch.equal(mem, before[1])
+    # a spliced matrix and its codes in one buffer, the codes in the columns beside it
+    s = torch.zeros(9, 256, dtype=torch.float32, device="cuda")
+    s[:, :40] = x
+    q2, scale2 = int8.quantize_rows(s[:, :40], (-1, 0, 1), out=(s.view(torch.int8)[1:8, 160:280], torch.empty(7, device="cuda")))
+    q3, scale3 = int8.quantize_rows(x, (-1, 0, 1))
+    assert torch.equal(q2, q3) and torch.equal(scale2, scale3)

@@ -216,3 +216,56 @@ def test_weights_of_more_than_an_int_are_refused(shape):
     w = torch.zeros(1, dtype=torch.int8).expand(shape).as_subclass(OnGpu)
     with pytest.raises(KamdError, match="weight: %d x %d is too large" % shape):
         int8.AffineInt8(w, torch.ones(1).expand(shape[0]))
+
+
+def test_overlapping_memory_is_found():
+    """kamd::RowsMeet against the bytes themselves"""
+    class Rows(C.Structure):
+        _fields_ = [("p", C.c_void_p), ("ld", C.c_int64), ("width", C.c_int64), ("rows", C.c_int64)]
+    meet = lib()["_ZN4kamd8RowsMeetERKNS_10MemoryRowsES2_"]
+    meet.restype, meet.argtypes = C.c_bool, [C.POINTER(Rows), C.POINTER(Rows)]
+    rng = np.random.default_rng(7)
+
+    def draw(same_ld):
+        rows, ld = int(rng.integers(1, 7)), same_ld or int(rng.integers(1, 24))
+        return int(rng.integers(1000, 1090)), ld, int(rng.integers(1, ld + 1)) if rows > 1 else int(rng.integers(1, 40)), rows
+
+    def touched(p, ld, width, rows):
+        return {p + i * ld + j for i in range(rows) for j in range(width)}
+    seen = [0, 0]
+    for i in range(20000):
+        same = int(rng.integers(1, 24)) if i % 2 else 0
+        a, b = draw(same), draw(same)
+        want = bool(touched(*a) & touched(*b))
+        seen[want] += 1
+        assert bool(meet(Rows(*a), Rows(*b))) == want, (a, b)
+    assert min(seen) > 4000
+    far = 1 << 46                                     # distances past 32 bits, and 2^30 rows of the same matrix
+    assert meet(Rows(far, 1 << 20, 64, 1 << 30), Rows(far + (1 << 50) - (1 << 20) + 63, 1 << 20, 4, 2))
+    assert not meet(Rows(far, 1 << 20, 64, 1 << 30), Rows(far + 64, 1 << 20, 64, 1 << 30))
+    assert not meet(Rows(None, 1, 1, 1), Rows(None, 1, 1, 1))
+
+
+def at(offset):
+    return C.c_void_p((1 << 20) + offset)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=at(4)), dict(out=at(0), ld_out=9), dict(out=at(4 * 8 * 3)), dict(out_type=BF16, type=BF16, out=at(2)),
+    dict(out=at(4096), sum=at(16), ld_sum=8), dict(out=at(4096), residual=at(8192), ld_r=8, sum=at(8192), ld_sum=10),
+    dict(out=at(4096), residual=at(8192 - 4), ld_r=8, sum=at(8192), ld_sum=8), dict(out=at(4096), sum=at(4096 + 4), ld_sum=8),
+    dict(out=at(4096), gain=at(4096 + 32)), dict(out=at(4096), gain=at(8192), sum=at(8192), ld_sum=8),
+    dict(out=at(0), out_type=I8, scale=at(4096)), dict(out=at(4096), out_type=I8, scale=at(4096 + 31)), dict(out=at(4096), out_type=I8, scale=at(12)),
+    dict(out=at(4096), out_type=I8, scale=at(8192), gain=at(8192 + 12)),
+])
+def test_rms_norm_refuses_overlaps(bad):
+    """an output that lies over another argument, but not exactly on a matrix of its type (4 rows of 8 are 128 bytes)"""
+    assert norm(**bad) == ERR_ARG
+    assert "overlaps" in lib().kamd_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [dict(q=at(0), scale=at(4096)), dict(q=at(127), scale=at(4096)), dict(q=at(4096), scale=at(124)), dict(q=at(4096), scale=at(4096 + 28)),
+                                 dict(q=at(4096), scale=at(4096 + 16), offsets=(0, 1))])
+def test_quantize_rows_refuses_overlaps(bad):
+    assert quantize(**bad) == ERR_ARG
+    assert "overlaps" in lib().kamd_last_error().decode()
