@@ -1,4 +1,4 @@
-// torch_int8.cc -- the calls of kaldi_amd/int8.py on torch tensors, as a Python extension module (kaldi_amd/lib/_torch_int8.so).
+// torch_int8.cc -- the calls of kaldi_amd/int8.py on torch tensors, as a Python extension module (kaldi_amd/lib/_torch_int8.*.so).
 //
 // A call on one frame takes the GPU 2 to 3 us; looked at from Python (attribute reads of four tensors, two allocations, sixteen
 // converted arguments) it took 9.  Here the same checks read the tensors themselves.  The work is the C-ABI's: the module is handed

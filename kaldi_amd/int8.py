@@ -13,13 +13,19 @@ calls on plain pointers.  Inference only: there are no gradients.
 import ctypes as C
 import importlib.util
 import os
+import sys
 
 import torch
 
 from ._lib import KamdError, lib
 
-_EXTENSION = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_torch_int8.so")
 _L = _X = None
+
+
+def _extension_path():
+    """the module that was built against this torch and this Python, whose tensors it reads (csrc/Makefile names it the same way)"""
+    name = "_torch_int8.%s.torch-%s.so" % (sys.implementation.cache_tag, torch.__version__)
+    return os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", name)
 
 
 def _library():
@@ -41,9 +47,10 @@ def _extension():
     global _X
     if _X is None:
         L = _library()
-        if not os.path.exists(_EXTENSION):
-            raise KamdError("%s is missing: run `python -c 'import __graft_entry__ as g; g.build()'`" % _EXTENSION)
-        spec = importlib.util.spec_from_file_location("_torch_int8", _EXTENSION)
+        path = _extension_path()
+        if not os.path.exists(path):
+            raise KamdError("%s is missing: run `python -c 'import __graft_entry__ as g; g.build()'`" % path)
+        spec = importlib.util.spec_from_file_location("_torch_int8", path)
         x = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(x)
         x.init(KamdError, torch._C._cuda_getCurrentRawStream,

@@ -3,8 +3,10 @@ import os
 import re
 import shutil
 import subprocess
+import sys
 
 import pytest
+import torch          # before the library: they share one HIP runtime then
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "kaldi_amd", "csrc")
@@ -56,3 +58,28 @@ def test_changed_settings_build_every_object(tree):
     assert objects(tree("KAMD_NT=512")) == objects(tree.everything)
     assert tree("KAMD_NT=512") == set()
     assert objects(tree()) == objects(tree.everything)
+
+
+def test_the_torch_module_is_of_one_torch(tree, tmp_path):
+    """it reads tensors through the layouts it was compiled with: another torch or Python gets a module of its own"""
+    from kaldi_amd import int8
+    name = os.path.basename(int8._extension_path())
+    assert name in tree.everything and os.path.exists(int8._extension_path())
+    other = tmp_path / "site" / "torch"
+    other.mkdir(parents=True)
+    (other / "__init__.py").write_text("")
+    (other / "version.py").write_text("__version__ = '99.1+x'\n")
+    python = tmp_path / "python"
+    python.write_text('#!/bin/sh\nPYTHONPATH=%s exec %s "$@"\n' % (other.parent, sys.executable))
+    python.chmod(0o755)
+    made = tree("PY=" + str(python))
+    assert len(made) == 1 and "torch-99.1+x" in made.pop()
+
+
+def test_a_module_of_another_torch_is_not_loaded(monkeypatch):
+    from kaldi_amd import int8
+    from kaldi_amd._lib import KamdError
+    monkeypatch.setattr(int8, "_X", None)
+    monkeypatch.setattr(torch, "__version__", "99.1+x")
+    with pytest.raises(KamdError, match="torch-99.1.*is missing"):
+        int8.rms_norm(torch.zeros(2, 8))
