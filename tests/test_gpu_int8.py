@@ -1,6 +1,9 @@
 """8-bit layers on the device (kaldi_amd.int8) against their formulas in 64 bits.
 
 Tolerances count roundings: u = 2^-24 is half a step of a 32-bit result; HALF[type] is half a step of the output's type."""
+import os
+import re
+
 import numpy as np
 import pytest
 import torch
@@ -628,3 +631,68 @@ def test_outputs_over_other_arguments_are_refused():
     q2, scale2 = int8.quantize_rows(s[:, :40], (-1, 0, 1), out=(s.view(torch.int8)[1:8, 160:280], torch.empty(7, device="cuda")))
     q3, scale3 = int8.quantize_rows(x, (-1, 0, 1))
     assert torch.equal(q2, q3) and torch.equal(scale2, scale3)
+
+
+# ---- each kernel of the product at the limits of what it addresses ---------------------------------------------------------
+
+def kernel_of(rows, k, n):
+    """The kernel that the cost rule of csrc/affine_i8.hip takes, (rows, channels, one to a CU) of its tile: the rule evaluated
+    with the constants that the source holds, so that a size that a new constant moves to another kernel is noticed."""
+    source = open(os.path.join(os.path.dirname(int8.__file__), "csrc", "affine_i8.hip")).read()
+    table = re.search(r"static const Kernel kernels\[\] = \{(.*?)\};", source, re.S).group(1)
+    kernels = re.findall(r"\{(\d+), (\d+), ([\d.]+), ([\d.]+), (true|false), Launch", table)
+    assert len(kernels) == 7
+    ceil = lambda a, b: -(-a // b)  # noqa: E731
+    best = None
+    for bm, bn, step, fixed, alone in kernels:
+        per_cu = ceil(ceil(rows, int(bm)) * ceil(n, int(bn)), 256)
+        cost = per_cu * (ceil(k, 128) * float(step) + float(fixed))
+        if not (alone == "true" and per_cu > 1) and (best is None or cost < best[0]):
+            best = cost, (int(bm), int(bn), alone == "true")
+    return best[1]
+
+
+def check_on_device(q, scale, w, ws, dtype, layer=None):
+    y = (layer or int8.AffineInt8(w, ws)).propagate(q, scale, dtype)
+    p = (q.double() @ w.double().T) * scale.double()[:, None] * ws.double()
+    off = (y.double() - p).abs() - p.abs() * (4 * U + HALF[dtype])               # the integer, two products, (and a bias of 0)
+    assert float(off.max()) <= TINY[dtype]
+
+
+def random_codes(rows, cols, seed, out=None):
+    g = torch.Generator("cuda").manual_seed(seed)
+    q = torch.randint(-127, 128, (rows, cols), generator=g, dtype=torch.int8, device="cuda")
+    return q if out is None else out.copy_(q)
+
+
+@pytest.mark.parametrize("rows, n, kernel", [(40, 50, (16, 16, False)), (300, 301, (32, 32, False)), (700, 701, (64, 64, False)), (1000, 1501, (64, 128, False)),
+                                             (2000, 2301, (128, 192, True)), (3000, 3501, (128, 192, False)), (4000, 4001, (256, 256, False))])
+def test_the_longest_sums_in_each_kernel(rows, n, kernel):
+    """131071 codes, the largest of them in some rows and channels: sums up to 2^31 - 16384, weights to the end of a descriptor"""
+    k = 131071
+    assert kernel_of(rows, k, n) == kernel
+    q, w = random_codes(rows, k, 81, int8.empty_codes(rows, k, "cuda")), random_codes(n, k, 82)
+    for t in (q, w):
+        t[0], t[1], t[-1], t[-2] = -128, 127, -128, 127
+    check_on_device(q, torch.rand(rows, device="cuda"), w, torch.rand(n, device="cuda"), torch.float32)
+
+
+@pytest.mark.parametrize("rows, k, n, kernel", [(200, 90, 300, (16, 16, False)), (300, 1000, 400, (32, 32, False)), (300, 1000, 1000, (64, 64, False)), (300, 500, 5000, (64, 128, False)),
+                                                (300, 1500, 16000, (128, 192, True)), (300, 100, 40001, (128, 192, False)), (512, 2000, 32767, (256, 256, False))])
+def test_rows_at_the_largest_distance_in_each_kernel(rows, k, n, kernel):
+    """rows of codes 2^23 bytes apart: a tile's rows end just below 2^31 from its first, the call's beyond 2^32"""
+    assert kernel_of(rows, k, n) == kernel
+    far = torch.empty(rows * (1 << 23), dtype=torch.int8, device="cuda").view(rows, 1 << 23)[:, :k]
+    random_codes(rows, k, 83, far)
+    check_on_device(far, torch.rand(rows, device="cuda"), random_codes(n, k, 84), torch.rand(n, device="cuda"), torch.bfloat16)
+    layer = int8.AffineInt8(random_codes(16, k, 85), torch.rand(16, device="cuda"))
+    with pytest.raises(KamdError, match="at most 8388608 apart"):
+        layer.propagate(torch.empty(2, (1 << 23) + 16, dtype=torch.int8, device="cuda")[:, :k], torch.rand(2, device="cuda"))
+
+
+@pytest.mark.parametrize("rows, k, n, kernel", [(9800, 700, 8190, (256, 256, False)), (8300, 700, 8200, (128, 192, False)), (600, 100, 120001, (128, 192, False))])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_16_bit_outputs_larger_than_the_caches(rows, k, n, kernel, dtype):
+    assert kernel_of(rows, k, n) == kernel and rows * n * 2 > 128 << 20
+    q, w = random_codes(rows, k, 86, int8.empty_codes(rows, k, "cuda")), random_codes(n, k, 87)
+    check_on_device(q, torch.rand(rows, device="cuda"), w, torch.rand(n, device="cuda") * 2.0 ** -12, dtype)
