@@ -261,10 +261,13 @@ enum { KAMD_F32 = 0, KAMD_BF16 = 1, KAMD_F16 = 2, KAMD_I8 = 3 };
 /* NormalizeComponent (nnet3/nnet-normalize-component.cc; NormalizePerRow, cudamatrix/cu-math.cc) with the residual and the
  * gain of a pre-norm layer, row by row:
  *   h = x (+ residual),   sum = h,   out = h / sqrt(mean(h^2) + eps) * gain
- * d_residual, d_gain (float [dim]; NULL = ones; constant target_rms = --target-rms) and d_sum may be NULL.  NormalizeComponent's
- * floor is eps = 2^-66.  h is the 32-bit sum, also where d_sum rounds it to 16 bits, and codes are made of the 32-bit h * gain.  out_type is `type`, or KAMD_I8: then out
- * holds codes in [-127, 127] and d_out_scale[row] their scale: out ~ code * scale, off by at most scale / 2; a row of zeros has
- * scale 0, one that holds an infinity or a NaN has scale NaN (and codes 0).  d_sum may be d_x or d_residual, and d_out (of the
+ * d_residual, d_gain (float [dim]; NULL = ones) and d_sum may be NULL.  For --target-rms=t every gain is t and eps is 2^-66 t^2:
+ * NormalizeComponent takes the larger of mean(h^2) and that floor where this call adds them, the same result for rows far above
+ * it and far below, smaller by up to a factor of sqrt(2) where the two are alike.  h is the 32-bit sum, also where d_sum rounds it to 16 bits.
+ * out_type is `type`, or KAMD_I8: then out holds codes in [-127, 127], made of the 32-bit h * gain, and d_out_scale[row] their
+ * scale: out ~ code * scale, off by at most scale / 2 and the roundings of 32-bit numbers (for rows below 2^-119, whose scale is
+ * a denormal number, its rounding too).  A row of zeros has scale 0; one in which an h * gain is an infinity (out of the 32-bit
+ * range included) or a NaN has scale NaN and codes 0.  d_sum may be d_x or d_residual, and d_out (of the
  * input's type) any of the three, at the same leading dimension; any other overlap of an output with another argument is refused,
  * here and in the calls below. */
 int kamd_rms_norm_device(const void *d_x, int64_t ld_x, const void *d_residual, int64_t ld_residual, int type,

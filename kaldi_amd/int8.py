@@ -69,14 +69,15 @@ def rms_norm(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
     (kamd_rms_norm_device).
 
     x: [rows, dim] float32 / bfloat16 / float16, rows any stride apart; residual: the same shape and type; gain: float32 [dim].
-    NormalizeComponent is gain = target_rms, eps = 2^-66.  sum_out (h) and out (y) may be given; sum_out may be x or residual,
+    NormalizeComponent with --target-rms=t is gain = t, eps = 2^-66 t^2, up to its floor: it takes the larger of mean(h^2) and eps
+    where this call adds them (the same far above and far below, by up to sqrt(2) smaller where they are alike).  sum_out (h) and out (y) may be given; sum_out may be x or residual,
     out any of the three.  Any other overlap of an output with another argument is refused, here and in the calls below."""
     return (_X or _extension()).rms_norm(x, gain, eps, residual, sum_out, out, False)
 
 
 def rms_norm_int8(x, gain=None, eps=1e-6, residual=None, sum_out=None, out=None):
     """rms_norm with y as 8-bit rows -> (codes, scale), or (codes, scale, h) with a residual or sum_out.  out = (codes, scale)
-    may be given."""
+    may be given.  A row in which an h * gain is not a finite 32-bit number has scale NaN and codes 0."""
     return (_X or _extension()).rms_norm(x, gain, eps, residual, sum_out, out, True)
 
 

@@ -696,3 +696,32 @@ def test_16_bit_outputs_larger_than_the_caches(rows, k, n, kernel, dtype):
     assert kernel_of(rows, k, n) == kernel and rows * n * 2 > 128 << 20
     q, w = random_codes(rows, k, 86, int8.empty_codes(rows, k, "cuda")), random_codes(n, k, 87)
     check_on_device(q, torch.rand(rows, device="cuda"), w, torch.rand(n, device="cuda") * 2.0 ** -12, dtype)
+
+
+@pytest.mark.parametrize("target", [1.0, 0.5, 3.0])
+def test_normalize_component_and_its_floor(target):
+    """NormalizeComponent's formula, x / sqrt(max(mean(x^2) / t^2, 2^-66)), in 64 bits (parity unpinned: there are no outputs of the
+    reference for it): equal far from the floor, at most sqrt(2) apart at it"""
+    dim, eps = 300, 2.0 ** -66 * target ** 2
+    level = torch.tensor([0.0, 2.0 ** -60, 2.0 ** -34, 2.0 ** -33, 2.0 ** -32, 2.0 ** -18, 1.0, 2.0 ** 40])[:, None]
+    x = rand(8, dim, seed=90)
+    x = x / x.double().square().mean(1, keepdim=True).sqrt().float() * level * target
+    want = x.double() / (x.double().square().mean(1, keepdim=True) / target ** 2).clamp_min(2.0 ** -66).sqrt()
+    y = int8.rms_norm(x.cuda(), torch.full((dim,), target, device="cuda"), eps).double().cpu()
+    # away from the floor: 1 / sqrt(1 + a), a <= 2^-30, beside the roundings of check_norm
+    far = [0, 1, 5, 6, 7]
+    assert bool(((y - want).abs()[far] <= want.abs()[far] * (6 * U + 2.0 ** -30)).all())
+    ratio = (want / y)[2:5][:, x[2].abs() > 0]
+    assert float(ratio.min()) >= 1 - 7 * U and float(ratio.max()) <= 2 ** 0.5 * (1 + 7 * U)
+    assert float(ratio[1].min()) > 1.41
+
+
+def test_a_gain_that_leaves_the_range_is_told():
+    """finite rows whose h * gain is none: codes of nothing under a NaN scale, in their row only"""
+    x = rand(3, 64, seed=91)
+    x[1, 5] = 2e38
+    gain = torch.full((64,), 4.0, device="cuda")
+    q, scale = int8.rms_norm_int8(x.cuda(), gain, EPS)
+    assert bool(torch.isnan(scale[1])) and int(q[1].abs().max()) == 0
+    check_codes(q[[0, 2]], scale[[0, 2]], norm64(x[[0, 2]], gain.cpu(), EPS)[1])
+    check_norm(int8.rms_norm(x.cuda(), gain, EPS), norm64(x, gain.cpu(), EPS)[1], torch.float32)
