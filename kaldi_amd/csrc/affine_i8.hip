@@ -441,8 +441,17 @@ int Propagate(AffineArgs p, hipStream_t st) {
   return KAMD_OK;
 }
 
+// For this thread, in this scope: allocating and freeing do not break a capture that is under way on some stream (a handle goes
+// when its last owner lets go of it, from the garbage collector perhaps, and hipFree would invalidate the capture and free nothing).
+struct OutsideCaptures {
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
 void Free(AffineI8 *c) {
   if (!c) return;
+  const OutsideCaptures guard;
   if (c->w) (void)hipFree(c->w);
   if (c->col) (void)hipFree(c->col);
   delete c;

@@ -725,3 +725,41 @@ def test_a_gain_that_leaves_the_range_is_told():
     assert bool(torch.isnan(scale[1])) and int(q[1].abs().max()) == 0
     check_codes(q[[0, 2]], scale[[0, 2]], norm64(x[[0, 2]], gain.cpu(), EPS)[1])
     check_norm(int8.rms_norm(x.cuda(), gain, EPS), norm64(x, gain.cpu(), EPS)[1], torch.float32)
+
+
+def test_a_handle_is_destroyed_while_a_stream_is_captured():
+    """by the capturing thread and by another one: the capture goes on, and the memory is given back"""
+    import threading
+
+    from kaldi_amd._lib import lib
+    n, k = 4096, 65536
+    w, ws, bias, _, _ = layer_of(64, 40, 92, True)
+    layer = int8.AffineInt8(w.cuda(), ws.cuda(), bias.cuda())
+    large = [int8.AffineInt8(torch.ones(1, 1, dtype=torch.int8, device="cuda").expand(n, k), torch.ones(n, device="cuda")) for _ in range(2)]
+    torch.cuda.empty_cache()
+    q, scale = on_device(codes(5, 64, 93)), torch.rand(5, device="cuda")
+    want = layer.propagate(q, scale)
+    torch.cuda.synchronize()
+
+    def free():
+        from ctypes import byref, c_size_t
+        f, t = c_size_t(), c_size_t()
+        assert lib().kamd_device_mem_info(byref(f), byref(t)) == 0
+        return f.value
+    before = free()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer.propagate(q, scale)
+        large.pop()
+        other = threading.Thread(target=large.clear)
+        other.start()
+        other.join()
+        z = layer.propagate(q, scale, torch.bfloat16)
+    for _ in range(3):
+        y.zero_()
+        z.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(z, want.bfloat16())
+    torch.cuda.empty_cache()
+    assert free() - before > n * k                                       # (both of them: 2 n k bytes, beside what the graph takes)
