@@ -457,6 +457,15 @@ void Free(AffineI8 *c) {
   delete c;
 }
 
+// A handle is filled here and now; a stream that is being captured does nothing now, and allocating would invalidate the capture.
+bool RefuseCapture(const char *who, hipStream_t st) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &status) == hipSuccess && status == hipStreamCaptureStatusNone) return false;
+  (void)hipGetLastError();
+  SetError(KAMD_ERR_STATE, "%s: the stream is being captured: layers are made before", who);
+  return true;
+}
+
 int CheckSizes(const char *who, int64_t in_dim, int64_t out_dim) {
   if (in_dim < 1 || out_dim < 1) return SetError(KAMD_ERR_ARG, "%s: bad sizes (%lld -> %lld)", who, static_cast<long long>(in_dim), static_cast<long long>(out_dim));
   if (in_dim > kMaxIn) return SetError(KAMD_ERR_ARG, "%s: %lld inputs: a 32-bit sum of 8-bit products holds at most %lld", who, static_cast<long long>(in_dim), static_cast<long long>(kMaxIn));
@@ -476,7 +485,7 @@ kamd_component_i8 *kamd_component_i8_create_quantized(const int8_t *d_w, int64_t
                                                       const float *d_bias, int relu, const float *d_mul, const float *d_add, void *stream) {
   if (kamd::CheckSizes("kamd_component_i8_create_quantized", in_dim, out_dim) != KAMD_OK) return NULL;
   if (!d_w || !d_w_scale || ld_w < in_dim) { SetError(KAMD_ERR_ARG, "kamd_component_i8_create_quantized: null argument or leading dimension smaller than the matrix"); return NULL; }
-  if (!kamd::RequireDevice()) return NULL;
+  if (!kamd::RequireDevice() || kamd::RefuseCapture("kamd_component_i8_create_quantized", static_cast<hipStream_t>(stream))) return NULL;
   AffineI8 *c = new (std::nothrow) AffineI8();
   if (!c) { SetError(KAMD_ERR_HIP, "kamd_component_i8_create_quantized: out of memory"); return NULL; }
   c->in_dim = in_dim; c->out_dim = out_dim; c->kp = kamd::RoundUp(in_dim, kamd::kPadK); c->np = kamd::RoundUp(out_dim, kamd::kPadN);
@@ -512,7 +521,7 @@ kamd_component_i8 *kamd_component_i8_create(const kamd_layer_desc *layer) {
   const size_t values = static_cast<size_t>(n) * k;
   for (size_t i = 0; i < values; i++)
     if (!std::isfinite(layer->W[i])) { SetError(KAMD_ERR_ARG, "kamd_component_i8_create: weight %zu is not finite", i); return NULL; }
-  if (!kamd::RequireDevice()) return NULL;
+  if (!kamd::RequireDevice() || kamd::RefuseCapture("kamd_component_i8_create", NULL)) return NULL;
   // weights, their codes and scales, and the channel vectors: one allocation, released below
   const size_t f_w = values, f_col = static_cast<size_t>(n) * 4, bytes = (f_w + f_col) * 4 + values;
   float *d = NULL;

@@ -98,7 +98,8 @@ class AffineInt8:
     """The affine layer on 8-bit rows (kamd_component_i8): out = mul * relu(codes @ weight.T * scale * weight_scale + bias) + add.
 
     weight: int8 [out_dim, in_dim], weight_scale: float32 [out_dim], both on the device; bias, mul, add: float32 [out_dim] or
-    None.  They are laid out for the matrix units once, here; the tensors are not kept."""
+    None.  They are laid out for the matrix units once, here (not while the stream is captured); the tensors are not kept.  A
+    layer has to live as long as the graphs that captured its calls."""
 
     def __init__(self, weight, weight_scale, bias=None, relu=False, mul=None, add=None):
         L = _library()
@@ -127,6 +128,8 @@ class AffineInt8:
         self = cls.__new__(cls)
         self._h = None
         with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise KamdError("AffineInt8: the stream is being captured: layers are made before")
             self.device, self.offsets = torch.device("cuda", torch.cuda.current_device()), tuple(layer.offsets)
             model = Model([layer], layer.in_dim, 0, 1, layer.out_dim)
             self._take(L.kamd_component_i8_create(model.descs()))

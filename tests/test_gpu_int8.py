@@ -763,3 +763,27 @@ def test_a_handle_is_destroyed_while_a_stream_is_captured():
         assert torch.equal(y, want) and torch.equal(z, want.bfloat16())
     torch.cuda.empty_cache()
     assert free() - before > n * k                                       # (both of them: 2 n k bytes, beside what the graph takes)
+
+
+def test_layers_are_not_made_while_the_stream_is_captured():
+    """refused without breaking the capture"""
+    w, ws, bias, _, _ = layer_of(64, 40, 94, True)
+    w, ws, bias = w.cuda(), ws.cuda(), bias.cuda()
+    layer = int8.AffineInt8(w, ws, bias)
+    q, scale = on_device(codes(5, 64, 95)), torch.rand(5, device="cuda")
+    want = layer.propagate(q, scale)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer.propagate(q, scale)
+        for make in (lambda: int8.AffineInt8(w, ws, bias), lambda: int8.AffineInt8.from_layer(Layer("c", 8, 4, [0], -1, np.ones((4, 8), np.float32)))):
+            with pytest.raises(KamdError, match="being captured"):
+                make()
+        z = layer.propagate(q, scale)
+    for _ in range(3):
+        y.zero_()
+        z.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(z, want)
+    assert torch.equal(int8.AffineInt8(w, ws, bias).propagate(q, scale), want)
