@@ -441,6 +441,13 @@ int Propagate(AffineArgs p, hipStream_t st) {
   return KAMD_OK;
 }
 
+// An error that is told to the caller, or of no consequence, is not left to be found as the thread's last one by whoever asks next
+// (torch does after each of its launches).
+hipError_t Told(hipError_t e) {
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
+}
+
 // For this thread, in this scope: allocating and freeing do not break a capture that is under way on some stream (a handle goes
 // when its last owner lets go of it, from the garbage collector perhaps, and hipFree would invalidate the capture and free nothing).
 struct OutsideCaptures {
@@ -452,8 +459,8 @@ struct OutsideCaptures {
 void Free(AffineI8 *c) {
   if (!c) return;
   const OutsideCaptures guard;
-  if (c->w) (void)hipFree(c->w);
-  if (c->col) (void)hipFree(c->col);
+  for (void *p : {static_cast<void *>(c->w), static_cast<void *>(c->col)})
+    if (p) Told(hipFree(p));
   delete c;
 }
 
@@ -502,7 +509,7 @@ kamd_component_i8 *kamd_component_i8_create_quantized(const int8_t *d_w, int64_t
     e = hipGetLastError();
   }
   if (e == hipSuccess) e = hipStreamSynchronize(st);             // the caller's arrays may go, and any stream may use the handle
-  if (e != hipSuccess) {
+  if (kamd::Told(e) != hipSuccess) {
     SetError(KAMD_ERR_HIP, "kamd_component_i8_create_quantized: %s", hipGetErrorString(e));
     kamd::Free(c);
     return NULL;
@@ -526,7 +533,7 @@ kamd_component_i8 *kamd_component_i8_create(const kamd_layer_desc *layer) {
   const size_t f_w = values, f_col = static_cast<size_t>(n) * 4, bytes = (f_w + f_col) * 4 + values;
   float *d = NULL;
   hipError_t e = hipMalloc(reinterpret_cast<void **>(&d), bytes);
-  if (e != hipSuccess) { SetError(KAMD_ERR_HIP, "kamd_component_i8_create: %s", hipGetErrorString(e)); return NULL; }
+  if (kamd::Told(e) != hipSuccess) { SetError(KAMD_ERR_HIP, "kamd_component_i8_create: %s", hipGetErrorString(e)); return NULL; }
   float *d_scale = d + f_w, *d_bias = d_scale + n, *d_mul = d_bias + n, *d_add = d_mul + n;
   int8_t *d_q = reinterpret_cast<int8_t *>(d_add + n);
   // BatchNorm and post maps: (bn_scale * z + bn_offset + post_offset) * post_scale
@@ -543,14 +550,14 @@ kamd_component_i8 *kamd_component_i8_create(const kamd_layer_desc *layer) {
     if (e == hipSuccess && mapped) e = hipMemcpy(d_mul, mul.data(), sizeof(float) * n, hipMemcpyHostToDevice);
     if (e == hipSuccess && mapped) e = hipMemcpy(d_add, add.data(), sizeof(float) * n, hipMemcpyHostToDevice);
     const int32_t zero = 0;
-    if (e != hipSuccess) SetError(KAMD_ERR_HIP, "kamd_component_i8_create: %s", hipGetErrorString(e));
+    if (kamd::Told(e) != hipSuccess) SetError(KAMD_ERR_HIP, "kamd_component_i8_create: %s", hipGetErrorString(e));
     else if (kamd_quantize_rows_device(d, k, KAMD_F32, n, static_cast<int>(k), &zero, 1, d_q, k, d_scale, NULL) == KAMD_OK)
       c = kamd_component_i8_create_quantized(d_q, k, d_scale, static_cast<int>(k), n, layer->bias ? d_bias : NULL, layer->relu, mapped ? d_mul : NULL,
                                              mapped ? d_add : NULL, NULL);
   } catch (const std::exception &) {
     SetError(KAMD_ERR_HIP, "kamd_component_i8_create: out of memory");
   }
-  (void)hipFree(d);
+  kamd::Told(hipFree(d));
   return c;
 }
 

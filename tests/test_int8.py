@@ -269,3 +269,65 @@ def test_rms_norm_refuses_overlaps(bad):
 def test_quantize_rows_refuses_overlaps(bad):
     assert quantize(**bad) == ERR_ARG
     assert "overlaps" in lib().kamd_last_error().decode()
+
+
+FAKE_HIP = r"""
+// stands in for the HIP runtime: a device on which the Nth allocation and everything after it fails
+#include <stddef.h>
+int last, left;
+static int result(int e) { if (e) last = e; return e; }
+int hipGetDeviceCount(int *n) { *n = 1; return result(0); }
+int hipGetDevice(int *d) { *d = 0; return result(0); }
+int hipStreamIsCapturing(void *s, int *status) { (void)s; *status = 0; return result(0); }
+int hipThreadExchangeStreamCaptureMode(int *m) { (void)m; return result(0); }
+int hipMalloc(void **p, size_t n) { (void)n; *p = left > 0 ? (void *)4096 : NULL; return result(left-- > 0 ? 0 : 2); }
+int hipFree(void *p) { (void)p; return result(1); }
+int hipHostMalloc(void **p, size_t n, unsigned f) { (void)n; (void)f; *p = NULL; return result(2); }
+int hipMemcpy(void *d, const void *s, size_t n, int k) { (void)d; (void)s; (void)n; (void)k; return result(2); }
+int hipMemcpyAsync(void *d, const void *s, size_t n, int k, void *st) { (void)d; (void)s; (void)n; (void)k; (void)st; return result(2); }
+int hipGetLastError(void) { int e = last; last = 0; return e; }
+int hipPeekAtLastError(void) { return last; }
+const char *hipGetErrorString(int e) { (void)e; return "out of memory"; }
+"""
+
+FAILED_LAYERS = r"""
+import ctypes as C, sys
+import numpy as np
+fake = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)          # before the library: its calls find these
+L = C.CDLL(sys.argv[2])
+from kaldi_amd import abi
+from kaldi_amd.nnet import Layer, Model
+L.kamd_component_i8_create_quantized.restype = L.kamd_component_i8_create.restype = C.c_void_p
+L.kamd_last_error.restype = C.c_char_p
+left, last, P = C.c_int.in_dll(fake, "left"), C.c_int.in_dll(fake, "last"), C.c_void_p(1 << 20)
+L.kamd_malloc.restype, L.kamd_malloc.argtypes = C.c_void_p, [C.c_size_t]
+assert L.kamd_malloc(64) is None and left.value == -1   # it is the stand-in that the library has
+fake.hipGetLastError()
+for n in (0, 1):
+    left.value = n
+    assert not L.kamd_component_i8_create_quantized(P, C.c_int64(8), P, 8, 4, None, 0, None, None, None)
+    assert b"out of memory" in L.kamd_last_error() and left.value == -1, L.kamd_last_error()
+    assert last.value == 0, (n, last.value)
+model = Model([Layer("a", 8, 4, [0], -1, np.ones((4, 8), np.float32))], 8, 0, 1, 4)
+for n in (0, 1):
+    left.value = n
+    assert not L.kamd_component_i8_create(model.descs())
+    assert b"out of memory" in L.kamd_last_error(), L.kamd_last_error()
+    assert last.value == 0, (n, last.value)
+print("fine")
+"""
+
+
+def test_a_layer_that_fails_leaves_no_error_behind(tmp_path):
+    """torch asks for the thread's last error after each of its launches: that of a call which has told it is not to be found there"""
+    import os
+    import subprocess
+    import sys
+
+    import kaldi_amd
+    (tmp_path / "fake.c").write_text(FAKE_HIP)
+    subprocess.check_call(["gcc", "-shared", "-fPIC", "-o", str(tmp_path / "fake.so"), str(tmp_path / "fake.c")])
+    root = os.path.dirname(os.path.abspath(kaldi_amd.__file__))
+    r = subprocess.run([sys.executable, "-c", FAILED_LAYERS, str(tmp_path / "fake.so"), os.path.join(root, "lib", "libkaldi_amd.so")], capture_output=True, text=True,
+                       cwd=os.path.dirname(root))
+    assert r.stdout == "fine\n", r.stderr
