@@ -279,7 +279,9 @@ int kamd_quantize_rows_device(const void *d_x, int64_t ld_x, int type, int64_t i
                               const int32_t *offsets, int n_offsets, int8_t *d_q, int64_t ld_q, float *d_scale,
                               void *stream);
 /* kamd_component (one fused affine layer) in 8 bits: out = map(sum_k q[row][k] w[n][k] * scale[row] * w_scale[n] + bias[n]),
- * map = the layer's ReLU, then its BatchNorm and post maps. */
+ * map = the layer's ReLU, then its BatchNorm and post maps.  A handle is made now: not on a stream that is being captured
+ * (KAMD_ERR_STATE).  It has to live as long as the graphs that captured its calls; destroying it waits for the device and leaves
+ * other captures alone. */
 typedef struct kamd_component_i8 kamd_component_i8;
 /* From a layer description (host float weights): the weights are coded per output channel here.  No multi_input, ivector,
  * log-softmax; the bypass is ignored as in kamd_component. */

@@ -174,8 +174,8 @@ __device__ inline void WaitBut(int stages) {
 }
 
 // Many rows: BM rows x BN channels per workgroup of WM x WN waves, operands by DMA into a ring of NST stages of 128 codes in LDS.
-// Large products are bound by the power that the matrix units draw: 16384 x 8192 x 8192 runs at 2.8 POP/s with the clock at
-// 1.9 GHz of 2.4 and the matrix units 66 % busy; the matrix instructions alone reach 4.6.  Sums of ~1536 codes keep them 45 % busy:
+// Large products are bound by the power that the matrix units draw: 16384 x 8192 x 8192 runs at 2.7 POP/s (816 us a call) with the
+// clock at 1.9 GHz of 2.4 and the matrix units 67 % busy; the matrix instructions alone reach 4.6.  Sums of ~1536 codes keep them 43 % busy:
 // a tile's first loads and its output take a third of its time, which the other tile on the CU covers in part.
 template <int BM, int BN, int WM, int WN, int NST, bool STREAM, typename TO>
 __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
@@ -212,8 +212,9 @@ __global__ __launch_bounds__(WM * WN * 64) void TileKernel(AffineArgs p) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
   };
   // Where several tiles share a CU, tiles next to each other along a row start at different places of the sum, which is exact in
-  // any order, so that not all of them ask for the same lines at once: 12000 x 1536 x 1536 36.3 -> 35.5 us, 600 x 6000 x 1536
-  // 13.9 -> 12.8.  Of no use to the other tiles, up to 3 % slower.
+  // any order, so that not all of them ask for the same lines at once.  With inputs that change from call to call, us:  600 x 6000 x
+  // 1536 13.2 -> 12.3, 40000 x 768 x 768 43.3 -> 41.1, but 12000 x 1536 x 1536 33.7 -> 34.8 and five other sizes 1 to 3 % slower.
+  // Of no use to the other tiles.
   const int steps = p.kb >> 1, start = BM == 128 && NST == 2 ? (tn & 7) * 3 % steps : 0;
   auto issue = [&](int kt, int stage, int first, int last) {     // loads first .. last - 1 of this wave's for a stage
     kt += start;
@@ -365,9 +366,11 @@ __global__ __launch_bounds__(256) void ColumnsKernel(const float *w_scale, const
   to[3 * np + i] = in && add ? add[i] : 0.0f;
 }
 
-// Weights that the L2s (8 x 4 MB) cannot hold until the next call pass them by where one tile of at most 16 rows reads them once
+// Weights that the L2s (8 x 4 MB) cannot hold until the next call pass them by where a split kernel reads them for at most 16 rows
 // (us from HBM, in brackets from the last-level cache):  1 x 8192 x 8192  13.7 -> 12.1 (11.1 -> 11.3),  16 x 8192 x 8192  14.6 -> 13.3
 // (11.9 -> 12.8).  Not from 24 rows on, 16.3 -> 15.1 (12.3 -> 14.6), nor smaller ones:  1 x 4096 x 4096  5.0 -> 4.8 (L2s 3.1 -> 4.5).
+// From some 12000 channels on the cost rule below, which counts no bytes, takes LDS tiles for such calls, which read the weights
+// through the caches:  1 x 16384 x 4096  11.6 (16 x 16 split 9.9),  1 x 65536 x 8192  96 (75).
 constexpr int64_t kL2Bytes = 32 << 20;
 
 template <int TI, int TJ, typename TO>
@@ -381,8 +384,9 @@ void LaunchSplit(AffineArgs p, hipStream_t st) {
 }
 
 // An output that the last-level cache (256 MB) could not keep for the next layer anyway goes past the caches, whose lines the
-// operands need more: 16384 x 8192 x 8192 to bf16 (268 MB) 791 us instead of 850, with the coding of its rows behind it 4.5 % less.
-// A smaller one does not: 12000 x 1536 x 1536 (37 MB) with the next layers behind it takes 2 % longer if it has to be fetched.
+// operands need more.  A smaller one does not: the next layer would have to fetch it.  256 x 256 tiles with the coding of the rows
+// behind them, us, kept -> past:  98 MB 80 -> 88,  134 MB 145 -> 149,  164 MB 199 -> 196,  201 MB 249 -> 234,  268 MB (16384 x 8192
+// x 8192) 893 -> 883, that product alone 830 -> 738.
 constexpr int64_t kStreamBytes = 128 << 20;
 
 template <int BM, int BN, int WM, int WN, int NST, typename TO>
@@ -396,15 +400,16 @@ void LaunchTile(AffineArgs p, hipStream_t st) {
 }
 
 // Which kernel.  A call takes about  2 us + c (s step + fixed),  c = tiles per CU, s = steps of 128 codes, with the two constants
-// of each kernel measured on MI355X; the cheapest is taken (over 200 random sizes within 0.5 % of the fastest of them in the mean).
-// What the kernels are for, each against its neighbour (us):
+// of each kernel measured on MI355X; the cheapest is taken.  Over 200 random sizes that is 1.3 % from the fastest of them in the
+// mean, 14 % at most in calls of over 5 us (12000 x 6000 x 256).  Bytes are not counted, see above.
+// What the kernels are for, each against its neighbour (us, in a loop over the same operands):
 //   16 x 16 split    1 x 4096 x 4096  3.1 (32 x 32  4.1)          20 x 320 x 7840  5.3 (7.5)
-//   32 x 32 split    24 x 6000 x 1536  3.7 (16 x 16  4.8)         64 x 4096 x 4096  6.9 (64 x 64  8.9)
-//   64 x 64, 4 st.   256 x 4096 x 4096  9.5   (64 x 128 12.1)     1000 x 768 x 768  4.0 (4.9)
-//   64 x 128, 3 st.  512 x 4096 x 4096  13.3  (64 x 64 15.7)
-//   128 x 192, 3 st. 1999 x 2328 x 1537 14.3  (64 x 128 16.6, 2 stages 16.4): one tile per CU, so that it can have all the LDS
-//   128 x 192, 2 st. 12000 x 1536 x 1536 35.5 (256 x 256 44.6, 3 stages 40.2): two tiles per CU cover each other's waits
-//   256 x 256, 2 st. 4096 x 4096 x 4096 54.1  (128 x 192 69.4)   16384 x 8192 x 8192  791 (921)
+//   32 x 32 split    24 x 6000 x 1536  3.7 (16 x 16  4.8)         64 x 4096 x 4096  6.8 (64 x 64  8.8)
+//   64 x 64, 4 st.   256 x 4096 x 4096  9.4   (64 x 128 11.6)     1000 x 768 x 768  4.0 (4.8)
+//   64 x 128, 3 st.  512 x 4096 x 4096  12.5  (64 x 64 14.1)      600 x 6000 x 1536  10.2 (128 x 192 11.2)
+//   128 x 192, 3 st. 1999 x 2328 x 1537 12.5  (64 x 128 14.7, 2 stages 13.6): one tile per CU, so that it can have all the LDS
+//   128 x 192, 2 st. 12000 x 1536 x 1536 32.4 (256 x 256 43.2, 3 stages 33.8): two tiles per CU cover each other's waits
+//   256 x 256, 2 st. 4096 x 4096 x 4096 52.3  (128 x 192 65.7)    16384 x 8192 x 8192  738 (881)
 constexpr int kCus = 256;
 
 constexpr int kMaxRows = 1 << 22;         // per launch: the grid of the smallest tile stays within its limit

@@ -528,7 +528,7 @@ __global__ __launch_bounds__(256, OCC) void TdnnGemmDmaKernel(GemmArgs p) {
 //   * M0 and the ring stage are scalar and compile-time (the k loop is unrolled by the three stages), so the fragment
 //     reads are ds_read_b128 with immediate offsets from four per-lane base addresses;
 //   * the epilogue is compiled per layer form (EF: bias / ReLU / BatchNorm / bypass / post offset / post scale) -- no
-//     neutral operands -- with packed fp32 instructions and fused multiply-adds for the BatchNorm and bypass terms
+//     neutral operands -- with fused multiply-adds for the BatchNorm and bypass terms
 //     (one rounding instead of two; within the 1e-4 of the nnet parity tests, and identical for every batch
 //     composition).
 // Same LDS image and k order as the second generation: the GEMM sums are bit-equal to it.

@@ -13,8 +13,9 @@
 // Numbers: h and t are 32-bit; squares are summed in 64 bits (a row of bf16 values near 1e20 has no 32-bit sum of squares, and
 // the conversion hides behind the loads); every output is rounded once.
 //
-// What bounds it: the bytes.  Each row is read once and stays in registers (up to 32 elements per thread) between the
-// reduction and the output; only rows longer than 32768 elements are read twice.
+// What bounds it: the bytes, for rows of some hundred columns and splices of up to 3 such pieces.  Each row is read once and stays in registers (up to 48
+// elements per thread) between the reduction and the output, rows longer than 32768 elements excepted, which are read twice, and
+// splices of many pieces, each of which is rounded up to a pass of all the row's threads (RunRows).
 #include <cfloat>
 #include <cmath>
 
@@ -265,6 +266,10 @@ static int LaunchRows(RowArgs a, hipStream_t st) {
 //   norm 12000 x 1536 f32   64 x 24  28.2   256 x 8 26.4                       norm 16384 x 8192 bf16  1024 x 8 181  512 x 16 186  1024 x 16 250
 //   codes of 40000 x (3 x 768) f32  64 x 40  43   256 x 16  64                 norm 1 x 1536 bf16  256 x 8  2.4   64 x 32  3.1
 //   codes of 20000 x 4096 bf16  256 x 16  38.5   512 x 8  44.3  (the codes' kernels take the smaller workgroup of equals)
+// Every piece of a splice is rounded up to a pass of the row's threads, which splices of many pieces pay for (us, and the time
+// of their bytes):  40000 x (5 x 768) f32  80 (56),  bf16  474 (43);  40000 x (5 x 40) bf16  28 (2.3),  x (7 x 40)  624 (2.9).  From 7
+// pieces of 16-bit rows on, from 5 on below 1024 rows or over 512 columns, no pair holds the row: 1024 threads read it twice.
+// Norm to codes of 16385 .. 32768 f32 columns: 1024 threads x 32 elements spill 3 registers;  4096 x 32768  172 us (135).
 template <typename T, typename TO, bool NORM>
 static int RunRows(const RowArgs &a, hipStream_t st) {
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
